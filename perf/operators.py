@@ -240,15 +240,12 @@ MU, LR, DECAY = 0.95, 0.02, 0.1
 
 
 def _plain_muon(st):
-    nesterov = st["case"]["nesterov"]
     g = torch.stack([t.float() for t in st["grad"]])
-    m = MU * torch.stack(st["momentum"]) + (1 - MU) * g
-    u = MU * m + (1 - MU) * g if nesterov else m
-    o = _plain_newton_schulz(u)
-    for i, (p, mom) in enumerate(zip(st["param"], st["momentum"])):
-        mom.copy_(m[i])
-        p.copy_(p.float() * (1 - LR * DECAY) - LR * o[i])
-    return [st["params"], st["momenta"]]
+    params, momenta = st["params"], st["momenta"]
+    momenta.copy_(MU * momenta + (1 - MU) * g)
+    u = MU * momenta + (1 - MU) * g if st["case"]["nesterov"] else momenta
+    params.copy_(params.float() * (1 - LR * DECAY) - LR * _plain_newton_schulz(u))
+    return [params, momenta]
 
 
 def run(state):
