@@ -52,7 +52,8 @@ typedef enum mhc_status {
   MHC_ERR_NO_DEVICE = 7,           /* no sm_100 device is current */
   MHC_ERR_LIMIT = 8,               /* a size beyond a fixed limit of the entry point */
   MHC_ERR_OUT_OF_BOUNDS = 9,       /* a debug-bounds build saw an access outside the call's buffers */
-  MHC_ERR_UNSUPPORTED = 10         /* the entry point is not compiled into this library */
+  MHC_ERR_UNSUPPORTED = 10,        /* the entry point is not compiled into this library */
+  MHC_ERR_OVERLAP = 11             /* buffers that have to be apart overlap */
 } mhc_status;
 
 /* Forward arguments.  Replaces the Python signature
@@ -314,6 +315,136 @@ typedef struct mhc_post_bwd_args {
 
 MHC_API int mhc_post_fwd(const mhc_post_fwd_args* args, void* stream);
 MHC_API int mhc_post_bwd(const mhc_post_bwd_args* args, void* stream);
+
+/* ------------------------------------------------- queries, keys, positions
+ * Norms of queries and keys for each head with the rotary position rotation
+ * in the same pass: what stands between the projection of h_in and the
+ * attention of a block's sublayer.  For a head row x [d] of token t, with
+ * s = row_scale[t] (1 when NULL) and w the side's weight (ones when NULL),
+ *   z = s x,  a = z w / sqrt(mean(z^2) + eps),  y = a with its first `rot`
+ *   elements turned by the angles position * inv_freq[i]: the pairs
+ *   (i, i + rot/2), or (2i, 2i + 1) when interleaved;  v_out = s v.
+ * row_scale takes h_in_rstd of mhc_fwd_ex: with the next norm's weight folded
+ * into the projection's columns, the projection runs on h_in itself.  No
+ * counterpart in the reference, which stops at h_in
+ * (src/forward/golden.py:62-63).
+ * Tensors are [batch, seq, heads, d] of `dtype` with unit stride along d and
+ * the given strides in elements; positions [batch, seq] are int32 or int64
+ * (position_bytes 4 or 8) or NULL, then 0 .. seq - 1.  Angles are exact to 32
+ * bits for |position| < 2^31.  1 <= d <= 1024, rot even and <= d; sums are 32
+ * bits wide.  No workspace in the forward; inputs and outputs do not overlap.
+ * 16-byte aligned tensors and strides with d and rot multiples of 16 and
+ * d <= 512 take the vector kernels (interleaved: any even rot). */
+typedef enum mhc_dtype { MHC_BF16 = 0, MHC_F16 = 1, MHC_F32 = 2 } mhc_dtype;
+
+/* A [batch, seq, heads, d] tensor: base pointer and the strides of its first
+ * three axes, in elements. */
+typedef struct mhc_heads {
+  void* data;
+  int64_t batch_stride;
+  int64_t seq_stride;
+  int64_t head_stride;
+} mhc_heads;
+
+typedef struct mhc_qk_args {
+  mhc_heads q, k, v;           /* v.data NULL: no values */
+  mhc_heads q_out, k_out, v_out;
+  const float* q_weight;       /* optional [d] */
+  const float* k_weight;       /* optional [d] */
+  const void* positions;       /* optional */
+  const float* inv_freq;       /* [rot / 2] */
+  const float* row_scale;      /* optional [batch, seq] */
+  int64_t position_batch_stride;
+  int64_t position_seq_stride;
+  int64_t batch;
+  int64_t seq;
+  int32_t q_heads, k_heads, v_heads;
+  int32_t d, rot;
+  int32_t position_bytes;
+  int32_t interleaved;
+  int32_t dtype;               /* mhc_dtype of q, k, v and the outputs */
+  float eps;
+} mhc_qk_args;
+
+/* Backward: `fwd` holds the forward's inputs (its outputs are ignored), dq_out,
+ * dk_out, dv_out the upstream gradients; dq, dk, dv receive the gradients of
+ * q, k, v, and the optional dq_weight, dk_weight [d], d_row_scale [batch, seq]
+ * those of the weights and the row factor.  Weight gradients are added in a
+ * fixed order: repeated calls return identical bytes.  The workspace need not
+ * be zeroed. */
+typedef struct mhc_qk_bwd_args {
+  mhc_qk_args fwd;
+  mhc_heads dq_out, dk_out, dv_out;
+  mhc_heads dq, dk, dv;
+  float* dq_weight;
+  float* dk_weight;
+  float* d_row_scale;
+  void* workspace;
+  size_t workspace_bytes;
+} mhc_qk_bwd_args;
+
+MHC_API int mhc_qk_norm_rope(const mhc_qk_args* args, void* stream);
+/* Workspace bytes of mhc_qk_norm_rope_bwd, 0 without weight gradients.  It
+ * depends on the current device's SM count. */
+MHC_API int mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t d, size_t* bytes);
+MHC_API int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------- updates of phi
+ * Newton-Schulz orthogonalisation of `count` matrices [rows, cols] (dense row
+ * major; min(rows, cols) <= 80, the n*n + 2n rows of phi for n <= 8):
+ *   X = U / (|U|_F + eps), then per step X <- a X + (b A + c A^2) X, A = X X^T.
+ * coeffs holds `steps` (1 to 16) triples a, b, c on the host.  The matrices'
+ * pointers are host arrays.  eps >= 1e-20.  The small iteration runs in 64
+ * bits, the application in 32; results do not depend on `count`.  The
+ * workspace need not be zeroed.  No counterpart in the reference. */
+typedef struct mhc_ortho_args {
+  const void* const* in;
+  void* const* out;            /* may be `in` */
+  int64_t count;
+  int32_t rows;
+  int32_t cols;
+  int32_t dtype;               /* MHC_F32 or MHC_BF16, in and out */
+  int32_t steps;
+  const double* coeffs;
+  double eps;
+  void* workspace;
+  size_t workspace_bytes;
+} mhc_ortho_args;
+
+/* The momentum update of `count` parameters around it, in place:
+ *   m <- mu m + (1 - mu) g;  u = mu m + (1 - mu) g when nesterov, else m
+ *   p <- (1 - lr weight_decay) p - lr scale orthogonalised(u).
+ * Momenta are fp32, gradients and parameters fp32 or bf16.  lr comes from
+ * lr_device (one float in device memory, read when the kernels run) when that
+ * is not NULL.  Buffers that overlap return MHC_ERR_OVERLAP (gradients may
+ * overlap each other: they are only read). */
+typedef struct mhc_muon_args {
+  void* const* params;
+  const void* const* grads;
+  float* const* momenta;
+  int64_t count;
+  int32_t rows;
+  int32_t cols;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+  int32_t nesterov;
+  int32_t steps;
+  const double* coeffs;
+  double eps;
+  float momentum;
+  float weight_decay;
+  float scale;
+  float lr;
+  const float* lr_device;
+  void* workspace;
+  size_t workspace_bytes;
+} mhc_muon_args;
+
+/* Workspace bytes of mhc_orthogonalize and mhc_muon_step for these sizes on
+ * the current device. */
+MHC_API int mhc_ortho_workspace_size(int64_t count, int32_t rows, int32_t cols, size_t* bytes);
+MHC_API int mhc_orthogonalize(const mhc_ortho_args* args, void* stream);
+MHC_API int mhc_muon_step(const mhc_muon_args* args, void* stream);
 
 /* Number of kernels this library has launched in this process (all devices,
  * all threads).  No counterpart in the reference; used to report launches. */

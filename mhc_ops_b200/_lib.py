@@ -74,6 +74,56 @@ class PostBwdArgs(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    """Mirror of ``mhc_heads``."""
+    _fields_ = [("data", _c_void_p), ("batch_stride", ctypes.c_int64), ("seq_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class QkArgs(ctypes.Structure):
+    """Mirror of ``mhc_qk_args``."""
+    _fields_ = [
+        ("q", Heads), ("k", Heads), ("v", Heads), ("q_out", Heads), ("k_out", Heads), ("v_out", Heads),
+        ("q_weight", _c_void_p), ("k_weight", _c_void_p), ("positions", _c_void_p), ("inv_freq", _c_void_p),
+        ("row_scale", _c_void_p),
+        ("position_batch_stride", ctypes.c_int64), ("position_seq_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int64), ("seq", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32), ("v_heads", ctypes.c_int32),
+        ("d", ctypes.c_int32), ("rot", ctypes.c_int32), ("position_bytes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+    ]
+
+
+class QkBwdArgs(ctypes.Structure):
+    """Mirror of ``mhc_qk_bwd_args``."""
+    _fields_ = [
+        ("fwd", QkArgs), ("dq_out", Heads), ("dk_out", Heads), ("dv_out", Heads), ("dq", Heads), ("dk", Heads),
+        ("dv", Heads), ("dq_weight", _c_void_p), ("dk_weight", _c_void_p), ("d_row_scale", _c_void_p),
+        ("workspace", _c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class OrthoArgs(ctypes.Structure):
+    """Mirror of ``mhc_ortho_args``."""
+    _fields_ = [
+        ("inp", _c_void_p), ("out", _c_void_p), ("count", ctypes.c_int64),
+        ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("dtype", ctypes.c_int32), ("steps", ctypes.c_int32),
+        ("coeffs", _c_void_p), ("eps", ctypes.c_double), ("workspace", _c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class MuonArgs(ctypes.Structure):
+    """Mirror of ``mhc_muon_args``."""
+    _fields_ = [
+        ("params", _c_void_p), ("grads", _c_void_p), ("momenta", _c_void_p), ("count", ctypes.c_int64),
+        ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32), ("nesterov", ctypes.c_int32), ("steps", ctypes.c_int32),
+        ("coeffs", _c_void_p), ("eps", ctypes.c_double), ("momentum", ctypes.c_float),
+        ("weight_decay", ctypes.c_float), ("scale", ctypes.c_float), ("lr", ctypes.c_float), ("lr_device", _c_void_p),
+        ("workspace", _c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol include/mhc_ops.h declares, with its ctypes signature.
 SIGNATURES = {
     "mhc_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -104,6 +154,14 @@ SIGNATURES = {
                                                   ctypes.POINTER(ctypes.c_size_t)]),
     "mhc_post_fwd": (ctypes.c_int, [ctypes.POINTER(PostFwdArgs), _c_void_p]),
     "mhc_post_bwd": (ctypes.c_int, [ctypes.POINTER(PostBwdArgs), _c_void_p]),
+    "mhc_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkArgs), _c_void_p]),
+    "mhc_qk_norm_rope_bwd_workspace_size": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32,
+                                                           ctypes.POINTER(ctypes.c_size_t)]),
+    "mhc_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(QkBwdArgs), _c_void_p]),
+    "mhc_ortho_workspace_size": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                                ctypes.POINTER(ctypes.c_size_t)]),
+    "mhc_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthoArgs), _c_void_p]),
+    "mhc_muon_step": (ctypes.c_int, [ctypes.POINTER(MuonArgs), _c_void_p]),
     "mhc_launch_count": (ctypes.c_uint64, []),
     "mhc_abi_version": (ctypes.c_int, []),
     "mhc_debug_bounds": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint64), ctypes.c_int]),
@@ -151,6 +209,17 @@ class MhcError(RuntimeError):
 def check(status: int, where: str) -> None:
     if status != MHC_OK:
         raise MhcError(status, where)
+
+
+# mhc_dtype of the tensors the newer entry points take
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Workspace of one call, from torch's allocator on the current stream: two
+    streams, host threads or captured graphs never share it (inside a capture
+    it belongs to the graph's own pool)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

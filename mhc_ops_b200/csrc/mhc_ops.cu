@@ -4,7 +4,9 @@
 // are in generic.cuh (any shape), fwd_sm100.cuh / bwd_sm100.cuh (tcgen05 +
 // TMA kernels for the shapes the tensor cores take), rowdot.cuh (the
 // streaming whole-row kernels beside them), tiled.cuh (the backward for n
-// other than 4) and post.cuh (the post-op that consumes h_post / h_res).
+// other than 4), post.cuh (the post-op that consumes h_post / h_res),
+// qkrope.cuh (per-head norms of queries and keys with the rotary rotation)
+// and ortho.cuh (Newton-Schulz orthogonalisation and the update of phi).
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -18,6 +20,7 @@
 #include <mutex>
 #include <set>
 #include <utility>
+#include <vector>
 
 #include "common.cuh"
 #include "generic.cuh"
@@ -27,6 +30,8 @@
 #include "rowdot.cuh"
 #include "tiled.cuh"
 #include "post.cuh"
+#include "qkrope.cuh"
+#include "ortho.cuh"
 
 #undef MHC_FILE_ID
 #define MHC_FILE_ID 7   // debug-bounds site ids: 7 * 100000 + line
@@ -1100,6 +1105,320 @@ struct PostBwd {
   }
 };
 
+// ------------------------------------------------- queries, keys, positions
+int rope_log2(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+rope::View rope_view(const mhc_heads& h) { return rope::View{h.data, h.batch_stride, h.seq_stride, h.head_stride}; }
+
+size_t dtype_bytes(int dtype) { return dtype == MHC_F32 ? 4 : 2; }
+
+bool rope_view_vec(const mhc_heads& h, size_t esize) {
+  const int64_t per16 = 16 / (int64_t)esize;
+  return !h.data || (aligned(h.data, 16) && h.batch_stride % per16 == 0 && h.seq_stride % per16 == 0 &&
+                     h.head_stride % per16 == 0);
+}
+
+// Largest element offset of a view, or -1 when a stride is negative or the
+// sum leaves 62 bits.
+int64_t rope_extent(const mhc_heads& h, int64_t B, int64_t S, int64_t H, int64_t d) {
+  if (h.batch_stride < 0 || h.seq_stride < 0 || h.head_stride < 0) return -1;
+  const __int128 e = (__int128)(B - 1) * h.batch_stride + (__int128)(S - 1) * h.seq_stride +
+                     (__int128)(H - 1) * h.head_stride + (d - 1);
+  return e > ((__int128)1 << 60) ? -1 : (int64_t)e;
+}
+
+// Shape and type checks shared by both directions.
+int rope_check(const mhc_qk_args* a) {
+  if (a->batch < 0 || a->seq < 0 || a->q_heads < 1 || a->k_heads < 1 || a->v_heads < 0 || a->q_heads > 4096 ||
+      a->k_heads > 4096 || a->v_heads > 4096 || a->d < 1 || a->d > rope::kMaxD || a->rot < 0 || a->rot > a->d ||
+      a->rot % 2 != 0 || a->dtype < 0 || a->dtype > 2 || !(a->eps >= 0.f))
+    return MHC_ERR_BAD_SHAPE;
+  if (a->seq > 0 && a->batch > (((int64_t)1 << 31) - 1) / a->seq) return MHC_ERR_BAD_SHAPE;
+  if (a->positions && a->position_bytes != 4 && a->position_bytes != 8) return MHC_ERR_BAD_SHAPE;
+  return MHC_OK;
+}
+
+// One tensor of the call: required, aligned to its elements, in range.
+int rope_check_view(const mhc_heads& h, const mhc_qk_args* a, int heads) {
+  if (!h.data) return MHC_ERR_NULL_POINTER;
+  if (!aligned(h.data, dtype_bytes(a->dtype))) return MHC_ERR_MISALIGNED;
+  return rope_extent(h, a->batch, a->seq, heads, a->d) < 0 ? MHC_ERR_BAD_SHAPE : MHC_OK;
+}
+
+struct RopePlan {
+  bool vec;
+  int blocks;
+  size_t smem;
+};
+
+// CTAs of the backward at most, so also rows of its weight-gradient partials.
+int rope_bwd_max_blocks(int sms) { return sms * 2; }
+
+RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, int sms) {
+  RopePlan r{};
+  p.q = rope_view(a->q);
+  p.k = rope_view(a->k);
+  p.v = rope_view(a->v);
+  p.wq = a->q_weight;
+  p.wk = a->k_weight;
+  p.inv_freq = a->inv_freq;
+  p.pos = a->positions;
+  p.pos64 = a->position_bytes == 8;
+  p.pos_sb = a->position_batch_stride;
+  p.pos_ss = a->position_seq_stride;
+  p.row_scale = a->row_scale;
+  p.T = a->batch * a->seq;
+  p.S = (int)a->seq;
+  p.Hq = a->q_heads;
+  p.Hk = a->k_heads;
+  p.Hv = a->v.data ? a->v_heads : 0;
+  p.d = a->d;
+  p.rot = a->rot;
+  p.eps = a->eps;
+  r.vec = vec_views && a->d % 16 == 0 && a->d <= 512 && (a->interleaved || a->rot % 16 == 0);
+  const int H = p.Hq + p.Hk + p.Hv;
+  p.gshift = r.vec ? rope_log2(a->d / 16) : 5;
+  p.G = 1 << p.gshift;
+  const int groups = (H + (32 >> p.gshift) - 1) / (32 >> p.gshift);
+  // Warps per token: one when the tokens alone fill the device (the angles are
+  // then computed once a token), more while there are few tokens.
+  p.parts = 1;
+  while (p.parts < rope::kWarps && p.parts < groups && p.T * p.parts < (int64_t)sms * rope::kWarps * 4) p.parts *= 2;
+  const int64_t tok_per_cta = rope::kWarps / p.parts;
+  const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
+  r.blocks = (int)std::min<int64_t>(want, backward ? rope_bwd_max_blocks(sms) : (int64_t)sms * 16);
+  r.smem = r.vec ? 0 : (size_t)rope::kWarps * (p.rot + (backward ? 2 * p.d : 0)) * sizeof(float);
+  return r;
+}
+
+template <class T, bool kInter>
+int rope_launch(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
+  if (backward) {
+    if (r.vec) {
+      rope::bwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, 0, s>>>(p);
+    } else {
+      MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_any_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(rope::kWarps * 3 * rope::kMaxD * sizeof(float))));
+      rope::bwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
+    }
+  } else if (r.vec) {
+    rope::fwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, 0, s>>>(p);
+  } else {
+    rope::fwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
+  }
+  return after_launch();
+}
+
+int rope_dispatch(const mhc_qk_args* a, const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
+  switch (a->dtype * 2 + (a->interleaved ? 1 : 0)) {
+    case 0: return rope_launch<__nv_bfloat16, false>(p, r, backward, s);
+    case 1: return rope_launch<__nv_bfloat16, true>(p, r, backward, s);
+    case 2: return rope_launch<__half, false>(p, r, backward, s);
+    case 3: return rope_launch<__half, true>(p, r, backward, s);
+    case 4: return rope_launch<float, false>(p, r, backward, s);
+    default: return rope_launch<float, true>(p, r, backward, s);
+  }
+}
+
+// ------------------------------------------------------- updates of phi
+struct OrthoPlan {
+  int R, C, NB, slices, chunks_per_slice, mats;   // mats: matrices of one launch
+  int64_t rs, cs;
+  size_t part_bytes, q_off, total;
+};
+
+OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
+  OrthoPlan p{};
+  const bool tall = rows > cols;
+  p.R = tall ? cols : rows;
+  p.C = tall ? rows : cols;
+  p.rs = tall ? 1 : cols;
+  p.cs = tall ? cols : 1;
+  p.NB = ortho::row_blocks(p.R);
+  p.mats = (int)std::min<int64_t>(count, ortho::kMaxMats);
+  const int kc = ortho::chunk_cols(p.NB);
+  const int chunks = (p.C + kc - 1) / kc;
+  // enough CTAs to fill the device a few times over, at most 32 partial sums
+  // for the iteration kernel's one CTA to add
+  int slices = (int)std::min<int64_t>({(int64_t)chunks, 32, (4 * (int64_t)sms + p.mats - 1) / std::max(1, p.mats)});
+  slices = std::max(1, slices);
+  p.chunks_per_slice = (chunks + slices - 1) / slices;
+  p.slices = (chunks + p.chunks_per_slice - 1) / p.chunks_per_slice;
+  p.part_bytes = (size_t)p.mats * p.slices * ortho::lower_blocks(p.NB) * 64 * sizeof(double);
+  p.q_off = align_up(p.part_bytes, kWsAlign);
+  p.total = align_up(p.q_off + (size_t)p.mats * 64 * p.NB * p.NB * sizeof(float), kWsAlign);
+  return p;
+}
+
+int ortho_check(int64_t count, int32_t rows, int32_t cols) {
+  if (count < 0 || count > 65536 || rows < 0 || cols < 0 || std::min(rows, cols) > ortho::kMaxRows ||
+      std::max(rows, cols) > (1 << 30))
+    return MHC_ERR_BAD_SHAPE;
+  return MHC_OK;
+}
+
+int ortho_check_coeffs(const double* coeffs, int32_t steps, double eps) {
+  if (!coeffs) return MHC_ERR_NULL_POINTER;
+  if (steps < 1 || steps > ortho::kMaxSteps || !(eps >= 1e-20)) return MHC_ERR_BAD_SHAPE;
+  return MHC_OK;
+}
+
+template <int NB, class T, class TO, bool kMom>
+int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, int mats, bool vec,
+                 cudaStream_t s) {
+  const dim3 grid(pl.slices, mats);
+  constexpr int gs = (int)ortho::gram_smem<NB>(), ns = (int)ortho::ns_smem<NB>();
+  constexpr int as = 64 * NB * NB * (int)sizeof(float2), cols = 2 * ortho::apply_threads(NB);
+  auto gram = vec ? ortho::gram_kernel<NB, T, kMom, true> : ortho::gram_kernel<NB, T, kMom, false>;
+  auto iterate = ortho::iterate_kernel<NB>;
+  auto apply = vec ? ortho::apply_kernel<NB, T, TO, kMom, true> : ortho::apply_kernel<NB, T, TO, kMom, false>;
+  MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
+  MHC_CUDA_TRY(cudaFuncSetAttribute(iterate, cudaFuncAttributeMaxDynamicSharedMemorySize, ns));
+  MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
+  int st;
+  gram<<<grid, ortho::kThreads, gs, s>>>(p, m);
+  if ((st = after_launch())) return st;
+  iterate<<<mats, ortho::kNsThreads, ns, s>>>(p);
+  if ((st = after_launch())) return st;
+  apply<<<dim3((pl.C + cols - 1) / cols, mats), ortho::apply_threads(NB), as, s>>>(p, m);
+  return after_launch();
+}
+
+template <class T, class TO, bool kMom>
+int ortho_dispatch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, int mats, bool vec,
+                   cudaStream_t s) {
+  switch (pl.NB) {
+    case 1: return ortho_launch<1, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 2: return ortho_launch<2, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 3: return ortho_launch<3, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 5: return ortho_launch<5, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 6: return ortho_launch<6, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 8: return ortho_launch<8, T, TO, kMom>(pl, p, m, mats, vec, s);
+    default: return ortho_launch<10, T, TO, kMom>(pl, p, m, mats, vec, s);
+  }
+}
+
+// Every list of a call, grads (or in) first, then outs (params), then momenta.
+struct OrthoLists {
+  const void* const* grads;
+  void* const* outs;
+  float* const* moms;   // NULL: orthogonalise only
+  int grad_dtype, out_dtype;
+};
+
+// No buffer that is written may share a byte with another one (MHC_ERR_OVERLAP).
+// `same` allows out[i] to be grads[i] itself.
+int ortho_overlap(const OrthoLists& l, int64_t count, size_t elems, bool same) {
+  struct Span {
+    uintptr_t lo, hi;
+    bool written;
+  };
+  std::vector<Span> v;
+  try {
+    v.reserve((size_t)count * 3);
+  } catch (...) {   // nothing may be thrown through a C entry point
+    return MHC_ERR_LIMIT;
+  }
+  for (int64_t i = 0; i < count; ++i) {
+    const uintptr_t g = reinterpret_cast<uintptr_t>(l.grads[i]), o = reinterpret_cast<uintptr_t>(l.outs[i]);
+    if (!(same && g == o)) v.push_back({g, g + elems * dtype_bytes(l.grad_dtype), false});
+    v.push_back({o, o + elems * dtype_bytes(l.out_dtype), true});
+    if (l.moms) {
+      const uintptr_t m = reinterpret_cast<uintptr_t>(l.moms[i]);
+      v.push_back({m, m + elems * 4, true});
+    }
+  }
+  std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t end = 0, end_written = 0;   // furthest ends of the spans before
+  for (const Span& x : v) {
+    if (x.lo < end_written || (x.written && x.lo < end)) return MHC_ERR_OVERLAP;
+    end = std::max(end, x.hi);
+    if (x.written) end_written = std::max(end_written, x.hi);
+  }
+  return MHC_OK;
+}
+
+#ifdef MHC_DEBUG_BOUNDS
+int dbg_register_list(const void* const* ptrs, const size_t* sizes, int count, cudaStream_t s);
+#endif
+
+int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Params& p, void* workspace, int sms,
+              cudaStream_t s) {
+  const OrthoPlan pl = ortho_plan(count, rows, cols, sms);
+  char* ws = static_cast<char*>(workspace);
+  p.R = pl.R;
+  p.C = pl.C;
+  p.rs = pl.rs;
+  p.cs = pl.cs;
+  p.slices = pl.slices;
+  p.chunks_per_slice = pl.chunks_per_slice;
+  p.part = reinterpret_cast<double*>(ws);
+  p.q = reinterpret_cast<float*>(ws + pl.q_off);
+  for (int64_t i0 = 0; i0 < count; i0 += pl.mats) {
+    const int mats = (int)std::min<int64_t>(pl.mats, count - i0);
+    ortho::Mats m{};
+    // pieces of four columns: rows that start on a multiple of four elements
+    bool vec = pl.cs == 1 && pl.C % 4 == 0;
+    for (int i = 0; i < mats; ++i) {
+      m.grad[i] = l.grads[i0 + i];
+      m.out[i] = l.outs[i0 + i];
+      m.mom[i] = l.moms ? l.moms[i0 + i] : nullptr;
+      vec = vec && aligned(m.grad[i], 4 * dtype_bytes(l.grad_dtype)) && aligned(m.out[i], 4 * dtype_bytes(l.out_dtype)) &&
+            aligned(m.mom[i], 16);
+    }
+#ifdef MHC_DEBUG_BOUNDS
+    {
+      const void* ptrs[3 * ortho::kMaxMats + 2];
+      size_t sizes[3 * ortho::kMaxMats + 2];
+      int n = 0;
+      const size_t elems = (size_t)rows * cols;
+      for (int i = 0; i < mats; ++i) {
+        ptrs[n] = m.grad[i], sizes[n++] = elems * dtype_bytes(l.grad_dtype);
+        ptrs[n] = m.out[i], sizes[n++] = elems * dtype_bytes(l.out_dtype);
+        ptrs[n] = m.mom[i], sizes[n++] = elems * 4;
+      }
+      ptrs[n] = ws, sizes[n++] = pl.total;
+      ptrs[n] = p.lr_dev, sizes[n++] = 4;
+      if (int st = dbg_register_list(ptrs, sizes, n, s)) return st;
+    }
+#endif
+    int st;
+    const bool gf = l.grad_dtype == MHC_F32, of = l.out_dtype == MHC_F32;
+    if (!l.moms)
+      st = gf ? ortho_dispatch<float, float, false>(pl, p, m, mats, vec, s)
+              : ortho_dispatch<uint16_t, uint16_t, false>(pl, p, m, mats, vec, s);
+    else if (gf)
+      st = of ? ortho_dispatch<float, float, true>(pl, p, m, mats, vec, s)
+              : ortho_dispatch<float, uint16_t, true>(pl, p, m, mats, vec, s);
+    else
+      st = of ? ortho_dispatch<uint16_t, float, true>(pl, p, m, mats, vec, s)
+              : ortho_dispatch<uint16_t, uint16_t, true>(pl, p, m, mats, vec, s);
+    if (st) return st;
+  }
+  return MHC_OK;
+}
+
+// Pointer, alignment and overlap checks of the lists, and of the workspace.
+int ortho_check_lists(const OrthoLists& l, int64_t count, int rows, int cols, bool same, const void* workspace,
+                      size_t workspace_bytes, int sms) {
+  if (!l.grads || !l.outs) return MHC_ERR_NULL_POINTER;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!l.grads[i] || !l.outs[i] || (l.moms && !l.moms[i])) return MHC_ERR_NULL_POINTER;
+    if (!aligned(l.grads[i], dtype_bytes(l.grad_dtype)) || !aligned(l.outs[i], dtype_bytes(l.out_dtype)) ||
+        (l.moms && !aligned(l.moms[i], 4)))
+      return MHC_ERR_MISALIGNED;
+  }
+  if (int st = ortho_overlap(l, count, (size_t)rows * cols, same)) return st;
+  if (!workspace) return MHC_ERR_NULL_POINTER;
+  if (!aligned(workspace, kWsAlign)) return MHC_ERR_MISALIGNED;
+  if (workspace_bytes < ortho_plan(count, rows, cols, sms).total) return MHC_ERR_WORKSPACE_TOO_SMALL;
+  return MHC_OK;
+}
+
 // The plan of mhc_query_plan / mhc_query_plan_for (shape already checked).
 int query_plan_impl(int which, int64_t tokens, int n, int D, int sms, bool fused_ok, int* path, int* cluster_size,
                     int* clusters) {
@@ -1147,6 +1466,7 @@ const char* mhc_status_string(int status) {
     case MHC_ERR_LIMIT: return "a size is beyond this entry point's fixed limit";
     case MHC_ERR_OUT_OF_BOUNDS: return "a debug-bounds build saw an access outside the call's buffers";
     case MHC_ERR_UNSUPPORTED: return "the entry point is not compiled into this library";
+    case MHC_ERR_OVERLAP: return "buffers that have to be apart overlap";
     default: return "unknown mhc status";
   }
 }
@@ -1247,6 +1567,46 @@ int dbg_register_post(const A* a, const void* const* ptrs, const size_t* sizes, 
   (void)a;
   DbgTable t;
   for (int i = 0; i < count; ++i) t.add(ptrs[i], sizes[i]);
+  return t.upload(s);
+}
+
+int dbg_register_list(const void* const* ptrs, const size_t* sizes, int count, cudaStream_t s) {
+  return dbg_register_post<void>(nullptr, ptrs, sizes, count, s);
+}
+
+// The bytes a [batch, seq, heads, d] view reaches.
+void dbg_add_view(DbgTable& t, const mhc_heads& h, const mhc_qk_args* a, int heads) {
+  if (h.data && heads > 0)
+    t.add(h.data, (size_t)(rope_extent(h, a->batch, a->seq, heads, a->d) + 1) * dtype_bytes(a->dtype));
+}
+
+int dbg_register_rope(const mhc_qk_args* a, const mhc_qk_bwd_args* b, cudaStream_t s) {
+  DbgTable t;
+  dbg_add_view(t, a->q, a, a->q_heads);
+  dbg_add_view(t, a->k, a, a->k_heads);
+  dbg_add_view(t, a->v, a, a->v_heads);
+  const size_t d = (size_t)a->d, T = (size_t)(a->batch * a->seq);
+  t.add(a->q_weight, d * 4);
+  t.add(a->k_weight, d * 4);
+  t.add(a->inv_freq, (size_t)a->rot / 2 * 4);
+  t.add(a->row_scale, T * 4);
+  if (a->positions)
+    t.add(a->positions, ((size_t)((a->batch - 1) * a->position_batch_stride + (a->seq - 1) * a->position_seq_stride) + 1) *
+                            a->position_bytes);
+  if (!b) {
+    dbg_add_view(t, a->q_out, a, a->q_heads);
+    dbg_add_view(t, a->k_out, a, a->k_heads);
+    if (a->v.data) dbg_add_view(t, a->v_out, a, a->v_heads);
+  } else {
+    for (const mhc_heads* h : {&b->dq_out, &b->dq}) dbg_add_view(t, *h, a, a->q_heads);
+    for (const mhc_heads* h : {&b->dk_out, &b->dk}) dbg_add_view(t, *h, a, a->k_heads);
+    if (a->v.data)
+      for (const mhc_heads* h : {&b->dv_out, &b->dv}) dbg_add_view(t, *h, a, a->v_heads);
+    t.add(b->dq_weight, d * 4);
+    t.add(b->dk_weight, d * 4);
+    t.add(b->d_row_scale, T * 4);
+    t.add(b->workspace, b->workspace_bytes);
+  }
   return t.upload(s);
 }
 
@@ -1512,6 +1872,158 @@ int mhc_post_bwd(const mhc_post_bwd_args* a, void* stream) {
   }
 #endif
   return dispatch_n<PostBwd>(a->n, a, static_cast<cudaStream_t>(stream), sms);
+}
+
+int mhc_qk_norm_rope(const mhc_qk_args* a, void* stream) {
+  if (!a) return MHC_ERR_NULL_POINTER;
+  int st = rope_check(a);
+  if (st) return st;
+  int sms = 0;
+  if ((st = current_sm_count(&sms))) return st;
+  if (a->batch == 0 || a->seq == 0) return MHC_OK;
+  if ((a->rot > 0 && !a->inv_freq)) return MHC_ERR_NULL_POINTER;
+  if ((st = rope_check_view(a->q, a, a->q_heads)) || (st = rope_check_view(a->k, a, a->k_heads)) ||
+      (st = rope_check_view(a->q_out, a, a->q_heads)) || (st = rope_check_view(a->k_out, a, a->k_heads)))
+    return st;
+  if (a->v.data && a->v_heads > 0 &&
+      ((st = rope_check_view(a->v, a, a->v_heads)) || (st = rope_check_view(a->v_out, a, a->v_heads))))
+    return st;
+  if (!aligned(a->q_weight, 4) || !aligned(a->k_weight, 4) || !aligned(a->inv_freq, 4) || !aligned(a->row_scale, 4) ||
+      (a->positions && !aligned(a->positions, a->position_bytes)))
+    return MHC_ERR_MISALIGNED;
+  const size_t es = dtype_bytes(a->dtype);
+  const bool vec = rope_view_vec(a->q, es) && rope_view_vec(a->k, es) && rope_view_vec(a->v, es) &&
+                   rope_view_vec(a->q_out, es) && rope_view_vec(a->k_out, es) &&
+                   (!a->v.data || rope_view_vec(a->v_out, es));
+  rope::Params p{};
+  const RopePlan r = rope_plan(a, p, vec, false, sms);
+  p.oq = rope_view(a->q_out);
+  p.ok = rope_view(a->k_out);
+  p.ov = rope_view(a->v_out);
+#ifdef MHC_DEBUG_BOUNDS
+  if ((st = dbg_register_rope(a, nullptr, static_cast<cudaStream_t>(stream)))) return st;
+#endif
+  return rope_dispatch(a, p, r, false, static_cast<cudaStream_t>(stream));
+}
+
+int mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t d, size_t* bytes) {
+  if (!bytes) return MHC_ERR_NULL_POINTER;
+  if (tokens < 0 || d < 1 || d > rope::kMaxD) return MHC_ERR_BAD_SHAPE;
+  int sms = 0;
+  if (int st = current_sm_count(&sms)) return st;
+  *bytes = (size_t)std::min<int64_t>(std::max<int64_t>(tokens, 1), rope_bwd_max_blocks(sms)) * 2 * d * sizeof(float);
+  return MHC_OK;
+}
+
+int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* b, void* stream) {
+  if (!b) return MHC_ERR_NULL_POINTER;
+  const mhc_qk_args* a = &b->fwd;
+  int st = rope_check(a);
+  if (st) return st;
+  int sms = 0;
+  if ((st = current_sm_count(&sms))) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!aligned(b->dq_weight, 4) || !aligned(b->dk_weight, 4) || !aligned(b->d_row_scale, 4)) return MHC_ERR_MISALIGNED;
+  if (a->batch == 0 || a->seq == 0) {   // sums over no tokens
+    if (b->dq_weight) MHC_CUDA_TRY(cudaMemsetAsync(b->dq_weight, 0, sizeof(float) * a->d, s));
+    if (b->dk_weight) MHC_CUDA_TRY(cudaMemsetAsync(b->dk_weight, 0, sizeof(float) * a->d, s));
+    return MHC_OK;
+  }
+  if ((a->rot > 0 && !a->inv_freq)) return MHC_ERR_NULL_POINTER;
+  for (const mhc_heads* h : {&a->q, &b->dq_out, &b->dq})
+    if ((st = rope_check_view(*h, a, a->q_heads))) return st;
+  for (const mhc_heads* h : {&a->k, &b->dk_out, &b->dk})
+    if ((st = rope_check_view(*h, a, a->k_heads))) return st;
+  const bool has_v = a->v.data && a->v_heads > 0;
+  if (has_v)
+    for (const mhc_heads* h : {&a->v, &b->dv_out, &b->dv})
+      if ((st = rope_check_view(*h, a, a->v_heads))) return st;
+  if (!aligned(a->q_weight, 4) || !aligned(a->k_weight, 4) || !aligned(a->inv_freq, 4) || !aligned(a->row_scale, 4) ||
+      (a->positions && !aligned(a->positions, a->position_bytes)))
+    return MHC_ERR_MISALIGNED;
+  const bool weights = b->dq_weight || b->dk_weight;
+  const size_t es = dtype_bytes(a->dtype);
+  bool vec = true;
+  for (const mhc_heads* h : {&a->q, &a->k, &b->dq_out, &b->dk_out, &b->dq, &b->dk}) vec = vec && rope_view_vec(*h, es);
+  if (has_v)
+    for (const mhc_heads* h : {&a->v, &b->dv_out, &b->dv}) vec = vec && rope_view_vec(*h, es);
+  rope::Params p{};
+  const RopePlan r = rope_plan(a, p, vec, true, sms);
+  if (weights) {
+    if (!b->workspace) return MHC_ERR_NULL_POINTER;
+    if (!aligned(b->workspace, 16)) return MHC_ERR_MISALIGNED;
+    if (b->workspace_bytes < (size_t)r.blocks * 2 * a->d * sizeof(float)) return MHC_ERR_WORKSPACE_TOO_SMALL;
+    p.dw_part = static_cast<float*>(b->workspace);
+  }
+  p.dq = rope_view(b->dq_out);
+  p.dk = rope_view(b->dk_out);
+  p.dv = rope_view(b->dv_out);
+  p.oq = rope_view(b->dq);
+  p.ok = rope_view(b->dk);
+  p.ov = rope_view(b->dv);
+  p.d_row_scale = b->d_row_scale;
+#ifdef MHC_DEBUG_BOUNDS
+  if ((st = dbg_register_rope(a, b, s))) return st;
+#endif
+  if ((st = rope_dispatch(a, p, r, true, s)) || !weights) return st;
+  rope::bwd_weights_kernel<<<(2 * a->d + rope::kFinCols - 1) / rope::kFinCols, rope::kThreads, 0, s>>>(
+      p.dw_part, r.blocks, a->d, b->dq_weight, b->dk_weight);
+  return after_launch();
+}
+
+int mhc_ortho_workspace_size(int64_t count, int32_t rows, int32_t cols, size_t* bytes) {
+  if (!bytes) return MHC_ERR_NULL_POINTER;
+  int st = ortho_check(count, rows, cols);
+  if (st) return st;
+  int sms = 0;
+  if ((st = current_sm_count(&sms))) return st;
+  *bytes = count == 0 || rows == 0 || cols == 0 ? 0 : ortho_plan(count, rows, cols, sms).total;
+  return MHC_OK;
+}
+
+int mhc_orthogonalize(const mhc_ortho_args* a, void* stream) {
+  if (!a) return MHC_ERR_NULL_POINTER;
+  int st = ortho_check(a->count, a->rows, a->cols);
+  if (st) return st;
+  if (a->dtype != MHC_F32 && a->dtype != MHC_BF16) return MHC_ERR_BAD_SHAPE;
+  if ((st = ortho_check_coeffs(a->coeffs, a->steps, a->eps))) return st;
+  int sms = 0;
+  if ((st = current_sm_count(&sms))) return st;
+  if (a->count == 0 || a->rows == 0 || a->cols == 0) return MHC_OK;
+  const OrthoLists l{a->in, a->out, nullptr, a->dtype, a->dtype};
+  if ((st = ortho_check_lists(l, a->count, a->rows, a->cols, true, a->workspace, a->workspace_bytes, sms))) return st;
+  ortho::Params p{};
+  p.steps = a->steps;
+  p.eps = a->eps;
+  std::copy(a->coeffs, a->coeffs + 3 * a->steps, p.coeffs);
+  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, sms, static_cast<cudaStream_t>(stream));
+}
+
+int mhc_muon_step(const mhc_muon_args* a, void* stream) {
+  if (!a) return MHC_ERR_NULL_POINTER;
+  int st = ortho_check(a->count, a->rows, a->cols);
+  if (st) return st;
+  for (int t : {a->param_dtype, a->grad_dtype})
+    if (t != MHC_F32 && t != MHC_BF16) return MHC_ERR_BAD_SHAPE;
+  if ((st = ortho_check_coeffs(a->coeffs, a->steps, a->eps))) return st;
+  int sms = 0;
+  if ((st = current_sm_count(&sms))) return st;
+  if (a->count == 0 || a->rows == 0 || a->cols == 0) return MHC_OK;
+  if (!a->momenta) return MHC_ERR_NULL_POINTER;
+  if (!aligned(a->lr_device, 4)) return MHC_ERR_MISALIGNED;
+  const OrthoLists l{a->grads, a->params, a->momenta, a->grad_dtype, a->param_dtype};
+  if ((st = ortho_check_lists(l, a->count, a->rows, a->cols, false, a->workspace, a->workspace_bytes, sms))) return st;
+  ortho::Params p{};
+  p.steps = a->steps;
+  p.eps = a->eps;
+  std::copy(a->coeffs, a->coeffs + 3 * a->steps, p.coeffs);
+  p.momentum = a->momentum;
+  p.nesterov = a->nesterov;
+  p.lr = a->lr;
+  p.lr_dev = a->lr_device;
+  p.decay = a->weight_decay;
+  p.scale = a->scale;
+  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, sms, static_cast<cudaStream_t>(stream));
 }
 
 int mhc_debug_bounds(uint64_t* record, int clear) {

@@ -51,12 +51,14 @@ class DataParallelMHC:
 
     ``backward(...)`` returns (dx_local, dphi, dalpha, dbias, dgamma) with the
     parameter gradients summed over all ranks (views into one flat buffer).
-    ``fwd`` / ``bwd`` are the forward and backward callables (the CUDA ones by
-    default); tests inject others to exercise the host logic on CPU ranks.
+    ``muon_step(...)`` then updates phi from them.  ``fwd`` / ``bwd`` / ``muon``
+    are the forward, backward and update callables (the CUDA ones by default);
+    tests inject others to exercise the host logic on CPU ranks.
     """
 
-    def __init__(self, n: int, D: int, group=None, fwd=None, bwd=None, device=None):
+    def __init__(self, n: int, D: int, group=None, fwd=None, bwd=None, device=None, muon=None):
         self.n, self.D, self.group = n, D, group
+        self.muon = muon
         if fwd is None or bwd is None:
             from .backward import mhc_backward_manual
             from .forward import mhc_forward_pre
@@ -106,3 +108,21 @@ class DataParallelMHC:
         if self.pending is not None:
             self.pending.wait()
             self.pending = None
+
+    def muon_step(self, phi, momentum, lr, **kw):
+        """The orthogonalised momentum update of phi (``mhc_muon_step``, whose
+        options ``kw`` takes), in place on ``phi`` and ``momentum``, from the
+        last ``backward``'s dphi: the sum over all ranks, an all-reduce left in
+        flight waited for first.  Every rank applies the same update to its
+        copy of phi; the kernels add in a fixed order, so the copies stay equal
+        bit for bit."""
+        if self.flat is None:
+            raise RuntimeError("muon_step needs the gradients of a backward first")
+        self.wait()
+        dphi = split_param_grads(self.flat, self.n, self.D)[0]
+        if tuple(phi.shape) != tuple(dphi.shape):
+            raise ValueError(f"phi must be {tuple(dphi.shape)}, got {tuple(phi.shape)}")
+        if self.muon is None:
+            from .muon import mhc_muon_step
+            self.muon = mhc_muon_step
+        self.muon(phi, dphi, momentum, lr, **kw)
