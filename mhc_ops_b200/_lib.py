@@ -211,17 +211,6 @@ def check(status: int, where: str) -> None:
         raise MhcError(status, where)
 
 
-# mhc_dtype of the tensors the newer entry points take
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-
-
-def scratch(nbytes: int, device: torch.device) -> torch.Tensor:
-    """Workspace of one call, from torch's allocator on the current stream: two
-    streams, host threads or captured graphs never share it (inside a capture
-    it belongs to the graph's own pool)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

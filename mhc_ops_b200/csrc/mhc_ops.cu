@@ -1183,7 +1183,8 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   const int H = p.Hq + p.Hk + p.Hv;
   p.gshift = r.vec ? rope_log2(a->d / 16) : 5;
   p.G = 1 << p.gshift;
-  const int groups = (H + (32 >> p.gshift) - 1) / (32 >> p.gshift);
+  const int hpw = 32 >> p.gshift;   // head rows a warp takes at a time, all of one side
+  const int groups = r.vec ? (p.Hq + hpw - 1) / hpw + (p.Hk + hpw - 1) / hpw + (p.Hv + hpw - 1) / hpw : H;
   // Warps per token: one when the tokens alone fill the device (the angles are
   // then computed once a token), more while there are few tokens.
   p.parts = 1;
@@ -1191,7 +1192,7 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   const int64_t tok_per_cta = rope::kWarps / p.parts;
   const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
   r.blocks = (int)std::min<int64_t>(want, backward ? rope_bwd_max_blocks(sms) : (int64_t)sms * 16);
-  r.smem = r.vec ? 0 : (size_t)rope::kWarps * (p.rot + (backward ? 2 * p.d : 0)) * sizeof(float);
+  r.smem = (size_t)rope::kWarps * sizeof(float) * (r.vec ? (backward ? 1024 : 0) : p.rot + (backward ? 2 * p.d : 0));
   return r;
 }
 
@@ -1199,7 +1200,10 @@ template <class T, bool kInter>
 int rope_launch(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
   if (backward) {
     if (r.vec) {
-      rope::bwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, 0, s>>>(p);
+      // with its static arrays more than a kernel has without asking
+      MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_vec_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)r.smem));
+      rope::bwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, p.dw_part ? r.smem : 0, s>>>(p);
     } else {
       MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_any_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)(rope::kWarps * 3 * rope::kMaxD * sizeof(float))));
@@ -1267,6 +1271,8 @@ int ortho_check_coeffs(const double* coeffs, int32_t steps, double eps) {
   return MHC_OK;
 }
 
+constexpr int kDefaultSmem = 48 * 1024;   // dynamic shared memory a kernel may have without asking
+
 template <int NB, class T, class TO, bool kMom>
 int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, int mats, bool vec,
                  cudaStream_t s) {
@@ -1276,9 +1282,9 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
   auto gram = vec ? ortho::gram_kernel<NB, T, kMom, true> : ortho::gram_kernel<NB, T, kMom, false>;
   auto iterate = ortho::iterate_kernel<NB>;
   auto apply = vec ? ortho::apply_kernel<NB, T, TO, kMom, true> : ortho::apply_kernel<NB, T, TO, kMom, false>;
-  MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
-  MHC_CUDA_TRY(cudaFuncSetAttribute(iterate, cudaFuncAttributeMaxDynamicSharedMemorySize, ns));
-  MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
+  if (gs > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
+  if (ns > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(iterate, cudaFuncAttributeMaxDynamicSharedMemorySize, ns));
+  if (as > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
   int st;
   gram<<<grid, ortho::kThreads, gs, s>>>(p, m);
   if ((st = after_launch())) return st;

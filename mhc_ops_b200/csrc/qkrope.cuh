@@ -63,8 +63,6 @@ struct Params {
   float eps;
 };
 
-__device__ __forceinline__ float to_f32(uint16_t v, __nv_bfloat16*) { return bf16_bits_to_f32(v); }
-
 template <class T>
 __device__ __forceinline__ float load1(const T* p) {
   if constexpr (std::is_same_v<T, float>) return MHC_LDG(p);
@@ -95,21 +93,20 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = MHC_LDG(reinterpret_cast<const uint4*>(p) + i);
   }
-  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+  __device__ __forceinline__ void unpack(float2 (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
       const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      if constexpr (std::is_same_v<T, float>) {
+        f[2 * i] = make_float2(__uint_as_float(u[0]), __uint_as_float(u[1]));
+        f[2 * i + 1] = make_float2(__uint_as_float(u[2]), __uint_as_float(u[3]));
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (std::is_same_v<T, float>) f[4 * i + j] = __uint_as_float(u[j]);
-        if constexpr (std::is_same_v<T, __half>) {
-          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
-          f[2 * j] = v.x;
-          f[2 * j + 1] = v.y;
-        }
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-          f[2 * j] = __uint_as_float(u[j] << 16);
-          f[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (std::is_same_v<T, __half>)
+            f[j] = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+          else
+            f[j] = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u));
         }
       }
     }
@@ -127,15 +124,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* p, const float2 (&f)[4]) {
   if constexpr (std::is_same_v<T, float>) {
-    MHC_ST(reinterpret_cast<uint4*>(p), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                                   __float_as_uint(f[3])));
-    MHC_ST(reinterpret_cast<uint4*>(p) + 1, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]),
-                                                       __float_as_uint(f[6]), __float_as_uint(f[7])));
+    MHC_ST(reinterpret_cast<float4*>(p), make_float4(f[0].x, f[0].y, f[1].x, f[1].y));
+    MHC_ST(reinterpret_cast<float4*>(p) + 1, make_float4(f[2].x, f[2].y, f[3].x, f[3].y));
   } else {
-    MHC_ST(reinterpret_cast<uint4*>(p),
-           make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])));
+    MHC_ST(reinterpret_cast<uint4*>(p), make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y),
+                                                   pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y)));
   }
 }
 
@@ -168,24 +163,28 @@ __device__ __forceinline__ void unit_offsets(int u, int rot, int& a, int& b) {
   }
 }
 
-// Rot (dir = 1) or its transpose (dir = -1: sn holds the negated sines) on a unit.
+// Two fp32 operations an instruction; each half rounds as the scalar one does.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 swapped(float2 v) { return make_float2(v.y, v.x); }
+
+// A turn of the pairs of a unit as x -> P x + Q x', x' the other element of
+// the pair: half-split pairs lie in the two chunks, interleaved ones side by side.
+struct Turn {
+  float2 pa[4], qa[4], pb[4], qb[4];
+};
 template <bool kInter>
-__device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const float (&cs)[8], const float (&sn)[8]) {
-  if constexpr (kInter) {
+__device__ __forceinline__ void apply_turn(const Turn& t, const float2 (&a)[4], const float2 (&b)[4], float2 (&ya)[4],
+                                           float2 (&yb)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a0 = a[2 * j], a1 = a[2 * j + 1], b0 = b[2 * j], b1 = b[2 * j + 1];
-      a[2 * j] = a0 * cs[j] - a1 * sn[j];
-      a[2 * j + 1] = a0 * sn[j] + a1 * cs[j];
-      b[2 * j] = b0 * cs[4 + j] - b1 * sn[4 + j];
-      b[2 * j + 1] = b0 * sn[4 + j] + b1 * cs[4 + j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = a[j], y = b[j];
-      a[j] = x * cs[j] - y * sn[j];
-      b[j] = x * sn[j] + y * cs[j];
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (kInter) {
+      ya[j] = fma2(swapped(a[j]), t.qa[j], mul2(a[j], t.pa[j]));
+      yb[j] = fma2(swapped(b[j]), t.qb[j], mul2(b[j], t.pb[j]));
+    } else {
+      ya[j] = fma2(b[j], t.qa[j], mul2(a[j], t.pa[j]));
+      yb[j] = fma2(a[j], t.qb[j], mul2(b[j], t.pb[j]));
     }
   }
 }
@@ -202,137 +201,190 @@ __device__ __forceinline__ const T* row(const View& v, int b, int s, int h) {
   return static_cast<const T*>(v.p) + (b * v.sb + s * v.ss + h * v.sh);
 }
 
-// Forward, 16-byte vectors.  A warp works on 32 / G heads of one token at a
-// time, G lanes a head with 16 elements each; its heads are the token's query,
-// key and value heads in one list, of which `parts` warps of the CTA take every
-// parts-th group.  The token's angles are computed once per warp.
-template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads) fwd_vec_kernel(const Params P) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = P.G, u = lane & (G - 1), hsub = lane >> P.gshift, hpw = 32 >> P.gshift;
-  const bool act = 16 * u < P.d;
-  int oa, ob;
-  unit_offsets<kInter>(u, P.rot, oa, ob);
-  float wq[2][8], wk[2][8];
+// What a lane of the vector kernels works on: G lanes a head row with 16
+// elements each, 32 / G head rows of one token and one side (queries, keys or
+// values) at a time.
+struct Lane {
+  int G, u, hsub, hpw, oa, ob;
+  bool act;
+  int ng[3];   // head groups of each side
+};
+template <bool kInter>
+__device__ __forceinline__ Lane lane_of(const Params& P) {
+  Lane l;
+  const int lane = threadIdx.x & 31;
+  l.G = P.G;
+  l.u = lane & (P.G - 1);
+  l.hsub = lane >> P.gshift;
+  l.hpw = 32 >> P.gshift;
+  l.act = 16 * l.u < P.d;
+  unit_offsets<kInter>(l.u, P.rot, l.oa, l.ob);
+  l.ng[0] = (P.Hq + l.hpw - 1) / l.hpw;
+  l.ng[1] = (P.Hk + l.hpw - 1) / l.hpw;
+  l.ng[2] = (P.Hv + l.hpw - 1) / l.hpw;
+  return l;
+}
+// Head group g of the token's list: its side and this lane's head.
+__device__ __forceinline__ int group_side(const Params& P, const Lane& l, int g, int& h, bool& in) {
+  const int side = g < l.ng[0] ? 0 : g < l.ng[0] + l.ng[1] ? 1 : 2;
+  const int g0 = side == 0 ? 0 : side == 1 ? l.ng[0] : l.ng[0] + l.ng[1];
+  h = (g - g0) * l.hpw + l.hsub;
+  in = l.act && h < (side == 0 ? P.Hq : side == 1 ? P.Hk : P.Hv);
+  return side;
+}
+
+// cos and sin of a token's rot / 2 angles into the warp's slots (ang[0] cos,
+// ang[1] sin; 1 and 0 up to the lanes' 8 per unit), each computed once a warp.
+__device__ __forceinline__ void token_angles(const Params& P, const Lane& l, int64_t pos, float (*ang)[256]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();   // the token before has been read
+  for (int i = lane; i < P.d / 2; i += 32) {
+    float c = 1.f, s = 0.f;
+    if (i < P.rot / 2) turn(pos, MHC_LDG(P.inv_freq + i), c, s);
+    ang[0][i] = c;
+    ang[1][i] = s;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void unit_angles(const float (*ang)[256], const Lane& l, float (&cs)[8], float (&sn)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    wq[0][j] = act && P.wq ? MHC_LDG(P.wq + oa + j) : 1.f;
-    wq[1][j] = act && P.wq ? MHC_LDG(P.wq + ob + j) : 1.f;
-    wk[0][j] = act && P.wk ? MHC_LDG(P.wk + oa + j) : 1.f;
-    wk[1][j] = act && P.wk ? MHC_LDG(P.wk + ob + j) : 1.f;
+    cs[j] = l.act ? ang[0][8 * l.u + j] : 1.f;
+    sn[j] = l.act ? ang[1][8 * l.u + j] : 0.f;
   }
-  const int H = P.Hq + P.Hk + P.Hv, Hqk = P.Hq + P.Hk;
+}
+
+// The unit's weights of a side from shared memory (ones without a weight).
+__device__ __forceinline__ void unit_weights(const float* sw, const Lane& l, float2 (&wa)[4], float2 (&wb)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    wa[j] = l.act ? *reinterpret_cast<const float2*>(sw + l.oa + 2 * j) : both(1.f);
+    wb[j] = l.act ? *reinterpret_cast<const float2*>(sw + l.ob + 2 * j) : both(1.f);
+  }
+}
+__device__ __forceinline__ void load_weights(const Params& P, float (*sw)[512]) {
+  for (int i = threadIdx.x; i < P.d; i += kThreads) {
+    sw[0][i] = P.wq ? MHC_LDG(P.wq + i) : 1.f;
+    sw[1][i] = P.wk ? MHC_LDG(P.wk + i) : 1.f;
+  }
+  __syncthreads();
+}
+
+// Forward, 16-byte vectors.  A warp takes a token's head groups (all of them,
+// or every parts-th), the next group's loads running during this one's
+// arithmetic.  The side's weights are folded into the turn's coefficients once
+// per token and side, so that a pair costs three packed instructions each way.
+template <class T, bool kInter>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fwd_vec_kernel(const Params P) {
+  __shared__ __align__(16) float sw[2][512];
+  __shared__ __align__(16) float angles[kWarps][2][256];
+  load_weights(P, sw);
+  const Lane l = lane_of<kInter>(P);
+  const int warp = threadIdx.x >> 5;
+  const int groups = l.ng[0] + l.ng[1] + l.ng[2];
   const float inv_d = 1.f / (float)P.d;
   const int part = warp & (P.parts - 1);
   const int tok_per_cta = kWarps / P.parts;
   for (int64_t t = (int64_t)blockIdx.x * tok_per_cta + warp / P.parts; t < P.T;
        t += (int64_t)gridDim.x * tok_per_cta) {
     const int b = (int)((uint32_t)t / (uint32_t)P.S), s = (int)((uint32_t)t - (uint32_t)b * (uint32_t)P.S);
-    const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
-    const int64_t pos = position(P, b, s);
-    auto locate = [&](int h, const T*& src, T*& dst) {
-      const bool isq = h < P.Hq, isk = !isq && h < Hqk;
-      const View& in = isq ? P.q : isk ? P.k : P.v;
-      const View& out = isq ? P.oq : isk ? P.ok : P.ov;
-      const int hh = isq ? h : isk ? h - P.Hq : h - Hqk;
-      src = row<T>(in, b, s, hh);
-      dst = const_cast<T*>(row<T>(out, b, s, hh));
+    auto fetch = [&](int g, Raw8<T>& ra, Raw8<T>& rb) {
+      int h;
+      bool in;
+      const int side = group_side(P, l, g, h, in);
+      ra.zero();
+      rb.zero();
+      if (g < groups && in) {
+        const T* src = row<T>(side == 0 ? P.q : side == 1 ? P.k : P.v, b, s, h);
+        ra.load(src + l.oa);
+        rb.load(src + l.ob);
+      }
     };
     Raw8<T> ra, rb;
-    const T* src;
-    T* dst;
-    int h = part * hpw + hsub;
-    ra.zero();
-    rb.zero();
-    if (h < H && act) {
-      locate(h, src, dst);
-      ra.load(src + oa);
-      rb.load(src + ob);
-    }
-    float cs[8], sn[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      cs[j] = 1.f;
-      sn[j] = 0.f;
-      if (8 * u + j < P.rot / 2) turn(pos, MHC_LDG(P.inv_freq + 8 * u + j), cs[j], sn[j]);
-    }
-    for (int h0 = part * hpw; h0 < H; h0 += P.parts * hpw) {
-      const int hn = h + P.parts * hpw;
+    fetch(part, ra, rb);
+    const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
+    token_angles(P, l, position(P, b, s), angles[warp]);
+    Turn tn;
+    int cur = -1;
+    for (int g = part; g < groups; g += P.parts) {
       Raw8<T> na, nb;
-      const T* nsrc;
-      T* ndst = nullptr;
-      na.zero();
-      nb.zero();
-      if (hn < H && act) {   // the next group's loads run during this one's arithmetic
-        locate(hn, nsrc, ndst);
-        na.load(nsrc + oa);
-        nb.load(nsrc + ob);
+      fetch(g + P.parts, na, nb);
+      int h;
+      bool in;
+      const int side = group_side(P, l, g, h, in);
+      if (side != cur && side < 2) {   // the same for the whole warp
+        cur = side;
+        float2 wa[4], wb[4];
+        float cs[8], sn[8];
+        unit_weights(sw[side], l, wa, wb);
+        unit_angles(angles[warp], l, cs, sn);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kInter) {
+            tn.pa[j] = mul2(wa[j], both(cs[j]));
+            tn.qa[j] = mul2(swapped(wa[j]), make_float2(-sn[j], sn[j]));
+            tn.pb[j] = mul2(wb[j], both(cs[4 + j]));
+            tn.qb[j] = mul2(swapped(wb[j]), make_float2(-sn[4 + j], sn[4 + j]));
+          } else {
+            const float2 c2 = make_float2(cs[2 * j], cs[2 * j + 1]), s2 = make_float2(sn[2 * j], sn[2 * j + 1]);
+            tn.pa[j] = mul2(wa[j], c2);
+            tn.qa[j] = mul2(wb[j], make_float2(-s2.x, -s2.y));
+            tn.pb[j] = mul2(wb[j], c2);
+            tn.qb[j] = mul2(wa[j], s2);
+          }
+        }
       }
-      float a[8], c[8];
+      float2 a[4], c[4], ya[4], yc[4];
       ra.unpack(a);
       rb.unpack(c);
-      float sq = 0.f;
+      float f = sc;
+      if (side < 2) {
+        float2 sq = mul2(a[0], a[0]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] *= sc;
-        c[j] *= sc;
-        sq = fmaf(a[j], a[j], sq);
-        sq = fmaf(c[j], c[j], sq);
+        for (int j = 1; j < 4; ++j) sq = fma2(a[j], a[j], sq);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sq = fma2(c[j], c[j], sq);
+        const float ms = group_sum(sq.x + sq.y, l.G) * inv_d;
+        f = sc * __frsqrt_rn(fmaf(ms * sc, sc, P.eps));
+        apply_turn<kInter>(tn, a, c, ya, yc);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ya[j] = a[j], yc[j] = c[j];
       }
-      sq = group_sum(sq, G);
-      if (h < Hqk) {
-        const float r = __frsqrt_rn(fmaf(sq, inv_d, P.eps));
-        const bool isq = h < P.Hq;
+      if (in) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          a[j] = a[j] * r * (isq ? wq[0][j] : wk[0][j]);
-          c[j] = c[j] * r * (isq ? wq[1][j] : wk[1][j]);
+        for (int j = 0; j < 4; ++j) {
+          ya[j] = mul2(ya[j], both(f));
+          yc[j] = mul2(yc[j], both(f));
         }
-        rotate<kInter>(a, c, cs, sn);
-      }
-      if (h < H && act) {
-        store8(dst + oa, a);
-        store8(dst + ob, c);
+        T* dst = const_cast<T*>(row<T>(side == 0 ? P.oq : side == 1 ? P.ok : P.ov, b, s, h));
+        store8(dst + l.oa, ya);
+        store8(dst + l.ob, yc);
       }
       ra = na;
       rb = nb;
-      dst = ndst;
-      h = hn;
     }
   }
 }
 
-// Sums of one warp's lanes of equal unit, over the head groups of the warp.
-__device__ __forceinline__ float across_heads(float v, int G) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    if (o >= G) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // Backward, 16-byte vectors, the forward's split.  Each lane keeps the weight
-// gradients of its 16 elements for queries and keys over all its tokens; the
-// CTA's warps are added in warp order and the CTA's row written for the
-// finalize kernel, so repeated calls give the same bits.
+// gradients of its 16 elements: in registers over a side's head groups, in its
+// own shared-memory slots over tokens.  The CTA's warps are added in warp order
+// and the CTA's row written for the finalize kernel, so repeated calls give the
+// same bits.
 template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads) bwd_vec_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const Params P) {
+  __shared__ __align__(16) float sw[2][512];
+  __shared__ __align__(16) float angles[kWarps][2][256];
   __shared__ float sds[kWarps];
-  __shared__ float sdw[kWarps][2][512];
+  extern __shared__ __align__(16) float dyn[];   // [kWarps][2][16][32] weight gradients, with dw_part only
+  load_weights(P, sw);
+  const Lane l = lane_of<kInter>(P);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = P.G, u = lane & (G - 1), hsub = lane >> P.gshift, hpw = 32 >> P.gshift;
-  const bool act = 16 * u < P.d;
-  int oa, ob;
-  unit_offsets<kInter>(u, P.rot, oa, ob);
-  float wq[2][8], wk[2][8], gq[2][8], gk[2][8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    wq[0][j] = act && P.wq ? MHC_LDG(P.wq + oa + j) : 1.f;
-    wq[1][j] = act && P.wq ? MHC_LDG(P.wq + ob + j) : 1.f;
-    wk[0][j] = act && P.wk ? MHC_LDG(P.wk + oa + j) : 1.f;
-    wk[1][j] = act && P.wk ? MHC_LDG(P.wk + ob + j) : 1.f;
-    gq[0][j] = gq[1][j] = gk[0][j] = gk[1][j] = 0.f;
-  }
-  const int H = P.Hq + P.Hk + P.Hv, Hqk = P.Hq + P.Hk;
+  float* gacc = dyn + warp * 1024 + lane;
+  if (P.dw_part)
+    for (int i = 0; i < 32; ++i) gacc[i * 32] = 0.f;
+  const int groups = l.ng[0] + l.ng[1] + l.ng[2];
   const float inv_d = 1.f / (float)P.d;
   const int part = warp & (P.parts - 1);
   const int tok_per_cta = kWarps / P.parts;
@@ -343,99 +395,120 @@ __global__ void __launch_bounds__(kThreads) bwd_vec_kernel(const Params P) {
     float ds = 0.f;
     if (t < P.T) {
       const int b = (int)((uint32_t)t / (uint32_t)P.S), s = (int)((uint32_t)t - (uint32_t)b * (uint32_t)P.S);
-      const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
-      const int64_t pos = position(P, b, s);
-      Raw8<T> xa, xb, ya, yb;
-      auto fetch = [&](int h, Raw8<T>& xa, Raw8<T>& xb, Raw8<T>& ya, Raw8<T>& yb) {
+      auto fetch = [&](int g, Raw8<T>& xa, Raw8<T>& xb, Raw8<T>& ya, Raw8<T>& yb) {
+        int h;
+        bool in;
+        const int side = group_side(P, l, g, h, in);
         xa.zero();
         xb.zero();
         ya.zero();
         yb.zero();
-        if (h < H && act) {
-          const bool isq = h < P.Hq, isk = !isq && h < Hqk;
-          const int hh = isq ? h : isk ? h - P.Hq : h - Hqk;
-          const T* x = row<T>(isq ? P.q : isk ? P.k : P.v, b, s, hh);
-          const T* y = row<T>(isq ? P.dq : isk ? P.dk : P.dv, b, s, hh);
-          xa.load(x + oa);
-          xb.load(x + ob);
-          ya.load(y + oa);
-          yb.load(y + ob);
+        if (g < groups && in) {
+          const T* x = row<T>(side == 0 ? P.q : side == 1 ? P.k : P.v, b, s, h);
+          const T* y = row<T>(side == 0 ? P.dq : side == 1 ? P.dk : P.dv, b, s, h);
+          xa.load(x + l.oa);
+          xb.load(x + l.ob);
+          ya.load(y + l.oa);
+          yb.load(y + l.ob);
         }
       };
-      int h = part * hpw + hsub;
-      fetch(h, xa, xb, ya, yb);
+      Raw8<T> xa, xb, ya, yb;
+      fetch(part, xa, xb, ya, yb);
+      const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
       float cs[8], sn[8];
+      token_angles(P, l, position(P, b, s), angles[warp]);
+      unit_angles(angles[warp], l, cs, sn);
+      float2 wa[4], wb[4], ga[4], gb[4];
+      int cur = -1;
+      auto flush = [&]() {   // the side's sums into the lane's slots
+        if (P.dw_part && cur >= 0) {
+          float* g = gacc + cur * 512;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cs[j] = 1.f;
-        sn[j] = 0.f;
-        if (8 * u + j < P.rot / 2) {
-          turn(pos, MHC_LDG(P.inv_freq + 8 * u + j), cs[j], sn[j]);
-          sn[j] = -sn[j];   // the transpose
+          for (int j = 0; j < 4; ++j) {
+            g[(2 * j) * 32] += ga[j].x;
+            g[(2 * j + 1) * 32] += ga[j].y;
+            g[(8 + 2 * j) * 32] += gb[j].x;
+            g[(8 + 2 * j + 1) * 32] += gb[j].y;
+          }
         }
-      }
-      for (int h0 = part * hpw; h0 < H; h0 += P.parts * hpw) {
+      };
+      for (int g = part; g < groups; g += P.parts) {
         Raw8<T> nxa, nxb, nya, nyb;
-        const int hn = h + P.parts * hpw;
-        fetch(hn, nxa, nxb, nya, nyb);
-        float x0[8], x1[8], y0[8], y1[8];
+        fetch(g + P.parts, nxa, nxb, nya, nyb);
+        int h;
+        bool in;
+        const int side = group_side(P, l, g, h, in);
+        float2 x0[4], x1[4], y0[4], y1[4], o0[4], o1[4];
         xa.unpack(x0);
         xb.unpack(x1);
         ya.unpack(y0);
         yb.unpack(y1);
-        const bool isq = h < P.Hq, isk = !isq && h < Hqk;
-        if (isq || isk) rotate<kInter>(y0, y1, cs, sn);   // da
-        float sq = 0.f, dot = 0.f;
+        if (side < 2) {
+          if (side != cur) {
+            flush();
+            cur = side;
+            unit_weights(sw[side], l, wa, wb);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float za = x0[j] * sc, zb = x1[j] * sc;
-          sq = fmaf(za, za, sq);
-          sq = fmaf(zb, zb, sq);
-          const float wa = isq ? wq[0][j] : isk ? wk[0][j] : 1.f, wb = isq ? wq[1][j] : isk ? wk[1][j] : 1.f;
-          dot = fmaf(y0[j] * wa, x0[j], dot);
-          dot = fmaf(y1[j] * wb, x1[j], dot);
-        }
-        sq = group_sum(sq, G);
-        dot = group_sum(dot, G);   // sum(dn x); sum(v dv_out) on value rows
-        float o0[8], o1[8];
-        if (isq || isk) {
-          const float r = __frsqrt_rn(fmaf(sq, inv_d, P.eps));
-          const float sr = sc * r;
-          const float m = sr * dot * inv_d;
-          if (u == 0) ds += P.eps * r * r * r * dot;
+            for (int j = 0; j < 4; ++j) ga[j] = gb[j] = both(0.f);
+          }
+          float2 d0[4], d1[4];   // da = Rot^T dy
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float n0 = x0[j] * sr, n1 = x1[j] * sr;
-            if (isq) {
-              gq[0][j] = fmaf(n0, y0[j], gq[0][j]);
-              gq[1][j] = fmaf(n1, y1[j], gq[1][j]);
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (kInter) {
+              d0[j] = fma2(swapped(y0[j]), make_float2(sn[j], -sn[j]), mul2(y0[j], both(cs[j])));
+              d1[j] = fma2(swapped(y1[j]), make_float2(sn[4 + j], -sn[4 + j]), mul2(y1[j], both(cs[4 + j])));
             } else {
-              gk[0][j] = fmaf(n0, y0[j], gk[0][j]);
-              gk[1][j] = fmaf(n1, y1[j], gk[1][j]);
+              const float2 c2 = make_float2(cs[2 * j], cs[2 * j + 1]), s2 = make_float2(sn[2 * j], sn[2 * j + 1]);
+              d0[j] = fma2(y1[j], s2, mul2(y0[j], c2));
+              d1[j] = fma2(y0[j], make_float2(-s2.x, -s2.y), mul2(y1[j], c2));
             }
-            o0[j] = sr * (y0[j] * (isq ? wq[0][j] : wk[0][j]) - n0 * m);
-            o1[j] = sr * (y1[j] * (isq ? wq[1][j] : wk[1][j]) - n1 * m);
+          }
+          float2 sq = both(0.f), dt = both(0.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sq = fma2(x0[j], x0[j], sq);
+            sq = fma2(x1[j], x1[j], sq);
+            y0[j] = mul2(d0[j], x0[j]);   // da x
+            y1[j] = mul2(d1[j], x1[j]);
+            dt = fma2(y0[j], wa[j], dt);
+            dt = fma2(y1[j], wb[j], dt);
+          }
+          const float ms = group_sum(sq.x + sq.y, l.G) * inv_d;
+          const float dot = group_sum(dt.x + dt.y, l.G);   // sum(dn x)
+          // a lane without a row adds nothing, whatever eps
+          const float r = in ? __frsqrt_rn(fmaf(ms * sc, sc, P.eps)) : 0.f;
+          const float sr = sc * r;
+          const float m2 = -sr * (sr * dot * inv_d);   // -s r m
+          if (l.u == 0) ds += P.eps * r * r * r * dot;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            ga[j] = fma2(y0[j], both(sr), ga[j]);
+            gb[j] = fma2(y1[j], both(sr), gb[j]);
+            o0[j] = mul2(both(sr), fma2(both(m2), x0[j], mul2(d0[j], wa[j])));
+            o1[j] = mul2(both(sr), fma2(both(m2), x1[j], mul2(d1[j], wb[j])));
           }
         } else {
-          if (u == 0) ds += dot;
+          float2 dt = both(0.f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            o0[j] = sc * y0[j];
-            o1[j] = sc * y1[j];
+          for (int j = 0; j < 4; ++j) {
+            dt = fma2(x0[j], y0[j], dt);
+            dt = fma2(x1[j], y1[j], dt);
+            o0[j] = mul2(both(sc), y0[j]);
+            o1[j] = mul2(both(sc), y1[j]);
           }
+          ds += dt.x + dt.y;
         }
-        if (h < H && act) {
-          const int hh = isq ? h : isk ? h - P.Hq : h - Hqk;
-          T* dst = const_cast<T*>(row<T>(isq ? P.oq : isk ? P.ok : P.ov, b, s, hh));
-          store8(dst + oa, o0);
-          store8(dst + ob, o1);
+        if (in) {
+          T* dst = const_cast<T*>(row<T>(side == 0 ? P.oq : side == 1 ? P.ok : P.ov, b, s, h));
+          store8(dst + l.oa, o0);
+          store8(dst + l.ob, o1);
         }
         xa = nxa;
         xb = nxb;
         ya = nya;
         yb = nyb;
-        h = hn;
       }
+      flush();
     }
     if (P.d_row_scale) {
       ds = warp_sum(ds);
@@ -454,23 +527,22 @@ __global__ void __launch_bounds__(kThreads) bwd_vec_kernel(const Params P) {
     }
   }
   if (P.dw_part) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v[4] = {across_heads(gq[0][j], G), across_heads(gq[1][j], G), across_heads(gk[0][j], G),
-                          across_heads(gk[1][j], G)};
-      if (hsub == 0 && act) {
-        sdw[warp][0][oa + j] = v[0];
-        sdw[warp][0][ob + j] = v[1];
-        sdw[warp][1][oa + j] = v[2];
-        sdw[warp][1][ob + j] = v[3];
-      }
-    }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * P.d; i += kThreads) {
       const int side = i >= P.d, col = i - side * P.d;
+      // the unit and the place in it that hold this column
+      int u, e;
+      if (!kInter && col < P.rot) {
+        const int half = P.rot / 2, c = col < half ? col : col - half;
+        u = c / 8;
+        e = (col < half ? 0 : 8) + c % 8;
+      } else {
+        u = col / 16;
+        e = col % 16;
+      }
       float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += sdw[w][side][col];
+      for (int w = 0; w < kWarps; ++w)
+        for (int k = 0; k < l.hpw; ++k) sum += dyn[w * 1024 + side * 512 + e * 32 + (k << P.gshift) + u];
       MHC_ST(P.dw_part + (int64_t)blockIdx.x * 2 * P.d + i, sum);
     }
   }

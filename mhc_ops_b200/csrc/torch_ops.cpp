@@ -11,6 +11,12 @@
 //     the reference's mhc_backward_manual (src/backward/golden.py:10-96;
 //     Triton call site src/backward/mhc_backward_triton.py:467-473).
 //
+//   mhc::qk_norm_rope, mhc::qk_norm_rope_bwd, mhc::qk_norm_rope_bwd_into,
+//   mhc::orthogonalize, mhc::muon_step_
+//     the operators around a training step that the reference has no
+//     counterpart of; schemas at the end of this file, semantics in
+//     include/mhc_ops.h.
+//
 // CUDA kernels convert tensors to the ABI's argument structs, allocate the
 // outputs, launch on at::cuda::getCurrentCUDAStream() and turn error codes
 // into TORCH_CHECK failures.  There is no CPU kernel: CPU tensors fail in the
@@ -28,22 +34,36 @@
 #include <cuda_runtime.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <map>
 #include <memory>
 #include <mutex>
+#include <string>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "mhc_ops.h"
 
 namespace {
+
+// Numbers go into messages as text: streaming one into a message aborted the
+// process where the installed torch and this library brought different C++
+// runtimes.
+std::string str(int64_t v) { return std::to_string(v); }
+std::string str(double v) { return std::to_string(v); }
+std::string str(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
 
 void check_cuda(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
 }
 
 void check_status(int st, const char* where) {
-  TORCH_CHECK(st == MHC_OK, where, ": mhc status ", st, ": ", mhc_status_string(st),
+  TORCH_CHECK(st == MHC_OK, where, ": mhc status ", str((int64_t)st), ": ", mhc_status_string(st),
               st == MHC_ERR_CUDA ? std::string(" (") + mhc_last_cuda_error() + ")" : std::string());
 }
 
@@ -141,7 +161,7 @@ void check_x(const at::Tensor& x) {
 }
 
 void check_shape(const at::Tensor& t, at::IntArrayRef want, const char* name) {
-  TORCH_CHECK(t.sizes() == want, name, " must be ", want, ", got ", t.sizes());
+  TORCH_CHECK(t.sizes() == want, name, " must be ", str(want), ", got ", str(t.sizes()));
 }
 
 }  // namespace
@@ -275,6 +295,385 @@ int64_t mhc_check_status() {
   return 0;
 }
 
+// ----------------------------------------------------------------- queries, keys, positions
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Scratch of one call, from torch's allocator on the current stream: two
+// streams, threads or captured graphs never share it.
+at::Tensor scratch(size_t nbytes, const at::Device& dev) {
+  return at::empty({(int64_t)nbytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+}
+
+int dtype_code(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return MHC_BF16;
+    case at::kHalf: return MHC_F16;
+    case at::kFloat: return MHC_F32;
+    default: return -1;
+  }
+}
+
+at::Tensor f32_of(const at::Tensor& t, const at::Device& dev, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), ", q is on ", dev);
+  return t.to(at::kFloat).contiguous();
+}
+
+mhc_heads heads_of(const at::Tensor& t) {
+  mhc_heads h{};
+  h.data = t.data_ptr();
+  h.batch_stride = t.stride(0);
+  h.seq_stride = t.stride(1);
+  h.head_stride = t.stride(2);
+  return h;
+}
+
+// A [B, S, heads, d] tensor of the call; heads < 0: any number.
+void check_heads(const at::Tensor& t, const char* name, const at::Tensor& like, int64_t heads) {
+  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be a tensor of shape [B, S, heads, d]");
+  TORCH_CHECK_TYPE(dtype_code(t) >= 0, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.size(0) == like.size(0) && t.size(1) == like.size(1) && t.size(3) == like.size(3) &&
+                        (heads < 0 || t.size(2) == heads),
+                    name, " must be [", str(like.size(0)), ", ", str(like.size(1)), ", ",
+                    heads < 0 ? std::string("heads") : str(heads), ", ", str(like.size(3)), "], got ", str(t.sizes()));
+  TORCH_CHECK_VALUE(t.scalar_type() == like.scalar_type() && t.device() == like.device(), name, " is ",
+                    t.scalar_type(), " on ", t.device(), ", expected ", like.scalar_type(), " on ", like.device());
+}
+
+at::Tensor unit_inner(const at::Tensor& t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+
+// The checked inputs of either direction and the tensors that own them.
+struct QkInputs {
+  mhc_qk_args a{};
+  at::Tensor q, k, v, inv_freq, q_weight, k_weight, row_scale;
+};
+
+QkInputs qk_inputs(const at::Tensor& q, const at::Tensor& k, const OptTensor& positions, const at::Tensor& inv_freq,
+                   const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& v,
+                   const OptTensor& row_scale, double eps, bool interleaved) {
+  QkInputs in;
+  check_heads(q, "q", q, -1);
+  check_heads(k, "k", q, -1);
+  const at::Device dev = q.device();
+  const int64_t B = q.size(0), S = q.size(1), d = q.size(3);
+  in.q = unit_inner(q);
+  in.k = unit_inner(k);
+  in.a.q = heads_of(in.q);
+  in.a.k = heads_of(in.k);
+  TORCH_CHECK_VALUE(d >= 1 && d <= 1024, "d must be at least 1 and at most 1024, got ", str(d));
+  TORCH_CHECK_VALUE(q.size(2) >= 1 && k.size(2) >= 1, "q and k need at least one head");
+  if (given(v)) {
+    check_heads(*v, "v", q, -1);
+    TORCH_CHECK_VALUE(v->size(2) >= 1, "v needs at least one head");
+    in.v = unit_inner(*v);
+    in.a.v = heads_of(in.v);
+    in.a.v_heads = (int32_t)v->size(2);
+  }
+  in.inv_freq = f32_of(inv_freq, dev, "inv_freq");
+  const int64_t rot = 2 * in.inv_freq.numel();
+  TORCH_CHECK_VALUE(in.inv_freq.dim() == 1 && rot <= d, "inv_freq must be [rot / 2] with rot <= d = ", str(d), ", got ",
+                    str(inv_freq.sizes()));
+  in.a.inv_freq = in.inv_freq.data_ptr<float>();
+  auto weight = [&](const OptTensor& w, const char* name, at::Tensor& keep, const float*& dst) {
+    if (!given(w)) return;
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == d, name, " must be [", str(d), "], got ", str(w->sizes()));
+    keep = f32_of(*w, dev, name);
+    dst = keep.data_ptr<float>();
+  };
+  weight(q_weight, "q_weight", in.q_weight, in.a.q_weight);
+  weight(k_weight, "k_weight", in.k_weight, in.a.k_weight);
+  if (given(row_scale)) {
+    TORCH_CHECK_VALUE(row_scale->dim() == 2 && row_scale->size(0) == B && row_scale->size(1) == S,
+                      "row_scale must be [", str(B), ", ", str(S), "], got ", str(row_scale->sizes()));
+    in.row_scale = f32_of(*row_scale, dev, "row_scale");
+    in.a.row_scale = in.row_scale.data_ptr<float>();
+  }
+  if (given(positions)) {
+    const at::Tensor& p = *positions;
+    TORCH_CHECK_TYPE(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong,
+                     "positions must be an int32 or int64 tensor");
+    TORCH_CHECK_VALUE(p.device() == dev, "positions is on ", p.device(), ", q is on ", dev);
+    if (p.dim() == 2 && p.size(0) == B && p.size(1) == S) {
+      in.a.position_batch_stride = p.stride(0);
+      in.a.position_seq_stride = p.stride(1);
+    } else {
+      TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == S, "positions must be [", str(B), ", ", str(S), "] or [", str(S),
+                        "], got ", str(p.sizes()));
+      in.a.position_seq_stride = p.stride(0);
+    }
+    in.a.positions = p.data_ptr();
+    in.a.position_bytes = (int32_t)p.element_size();
+  }
+  TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative, got ", str(eps));
+  in.a.batch = B;
+  in.a.seq = S;
+  in.a.q_heads = (int32_t)q.size(2);
+  in.a.k_heads = (int32_t)k.size(2);
+  in.a.d = (int32_t)d;
+  in.a.rot = (int32_t)rot;
+  in.a.interleaved = interleaved ? 1 : 0;
+  in.a.dtype = dtype_code(q);
+  in.a.eps = (float)eps;
+  return in;
+}
+
+at::Tensor empty_like_heads(const at::Tensor& t) { return at::empty(t.sizes(), t.options()); }
+
+// First byte and the byte behind the last one a strided tensor reaches.
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {lo, lo + (uintptr_t)(last + 1) * t.element_size()};
+}
+
+}  // namespace
+
+std::vector<at::Tensor> qk_norm_rope_cuda(const at::Tensor& q, const at::Tensor& k, const OptTensor& positions,
+                                          const at::Tensor& inv_freq, const OptTensor& q_weight,
+                                          const OptTensor& k_weight, const OptTensor& v, const OptTensor& row_scale,
+                                          double eps, bool interleaved) {
+  c10::cuda::CUDAGuard guard(q.device());
+  QkInputs in = qk_inputs(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps, interleaved);
+  std::vector<at::Tensor> out{empty_like_heads(q), empty_like_heads(k)};
+  in.a.q_out = heads_of(out[0]);
+  in.a.k_out = heads_of(out[1]);
+  if (in.v.defined()) {
+    out.push_back(empty_like_heads(in.v));
+    in.a.v_out = heads_of(out[2]);
+  }
+  check_status(mhc_qk_norm_rope(&in.a, at::cuda::getCurrentCUDAStream().stream()), "mhc::qk_norm_rope");
+  return out;
+}
+
+std::vector<at::Tensor> qk_norm_rope_bwd_into_cuda(
+    const at::Tensor& q, const at::Tensor& k, const OptTensor& positions, const at::Tensor& inv_freq,
+    const at::Tensor& dq_out, const at::Tensor& dk_out, const OptTensor& q_weight, const OptTensor& k_weight,
+    const OptTensor& v, const OptTensor& dv_out, const OptTensor& row_scale, double eps, bool interleaved,
+    bool weight_grads, bool row_scale_grad, at::TensorList grad_out) {
+  c10::cuda::CUDAGuard guard(q.device());
+  mhc_qk_bwd_args b{};
+  QkInputs in = qk_inputs(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps, interleaved);
+  TORCH_CHECK_VALUE(given(v) == given(dv_out), "v and dv_out go together");
+  const size_t count = given(v) ? 3 : 2;
+  static const char* const up_names[3] = {"dq_out", "dk_out", "dv_out"};
+  static const char* const grad_names[3] = {"grad_out dq", "grad_out dk", "grad_out dv"};
+  const at::Tensor inputs[3] = {in.q, in.k, in.v};
+  at::Tensor ups[3] = {dq_out, dk_out, given(dv_out) ? *dv_out : at::Tensor()};
+  mhc_heads* const up_dst[3] = {&b.dq_out, &b.dk_out, &b.dv_out};
+  mhc_heads* const grad_dst[3] = {&b.dq, &b.dk, &b.dv};
+  TORCH_CHECK_VALUE(grad_out.size() == count, "grad_out must hold ", str((int64_t)count), " tensors");
+  for (size_t i = 0; i < count; ++i) {
+    check_heads(ups[i], up_names[i], in.q, inputs[i].size(2));
+    ups[i] = unit_inner(ups[i]);
+    *up_dst[i] = heads_of(ups[i]);
+    const at::Tensor& g = grad_out[i];
+    check_heads(g, grad_names[i], in.q, inputs[i].size(2));
+    TORCH_CHECK_VALUE(g.size(3) == 1 || g.stride(3) == 1, grad_names[i], " must have unit stride along d");
+    for (int64_t j = 0; j < 3; ++j)
+      TORCH_CHECK_VALUE(g.stride(j) != 0 || g.size(j) <= 1, grad_names[i], " must not be an expanded tensor");
+    *grad_dst[i] = heads_of(g);
+  }
+  if (q.numel() > 0)
+    for (size_t i = 0; i < count; ++i) {
+      const auto w = span_of(grad_out[i]);
+      for (size_t j = 0; j < 2 * count; ++j) {
+        const auto r = span_of(j < count ? inputs[j] : ups[j - count]);
+        TORCH_CHECK_VALUE(w.first >= r.second || r.first >= w.second, grad_names[i], " overlaps an input");
+      }
+    }
+  std::vector<at::Tensor> out;
+  const auto f = q.options().dtype(at::kFloat);
+  if (in.q_weight.defined() && weight_grads) {
+    out.push_back(at::empty({q.size(3)}, f));
+    b.dq_weight = out.back().data_ptr<float>();
+  }
+  if (in.k_weight.defined() && weight_grads) {
+    out.push_back(at::empty({q.size(3)}, f));
+    b.dk_weight = out.back().data_ptr<float>();
+  }
+  if (in.row_scale.defined() && row_scale_grad) {
+    out.push_back(at::empty({q.size(0), q.size(1)}, f));
+    b.d_row_scale = out.back().data_ptr<float>();
+  }
+  at::Tensor ws;
+  if (b.dq_weight || b.dk_weight) {
+    check_status(mhc_qk_norm_rope_bwd_workspace_size(q.size(0) * q.size(1), in.a.d, &b.workspace_bytes),
+                 "mhc_qk_norm_rope_bwd_workspace_size");
+    ws = scratch(b.workspace_bytes, q.device());
+    b.workspace = ws.data_ptr();
+  }
+  b.fwd = in.a;
+  check_status(mhc_qk_norm_rope_bwd(&b, at::cuda::getCurrentCUDAStream().stream()), "mhc::qk_norm_rope_bwd");
+  return out;
+}
+
+std::vector<at::Tensor> qk_norm_rope_bwd_cuda(const at::Tensor& q, const at::Tensor& k, const OptTensor& positions,
+                                              const at::Tensor& inv_freq, const at::Tensor& dq_out,
+                                              const at::Tensor& dk_out, const OptTensor& q_weight,
+                                              const OptTensor& k_weight, const OptTensor& v, const OptTensor& dv_out,
+                                              const OptTensor& row_scale, double eps, bool interleaved,
+                                              bool weight_grads, bool row_scale_grad) {
+  c10::cuda::CUDAGuard guard(q.device());
+  std::vector<at::Tensor> grads{empty_like_heads(q), empty_like_heads(k)};
+  if (given(v)) grads.push_back(empty_like_heads(*v));
+  for (auto& t : qk_norm_rope_bwd_into_cuda(q, k, positions, inv_freq, dq_out, dk_out, q_weight, k_weight, v, dv_out,
+                                            row_scale, eps, interleaved, weight_grads, row_scale_grad, grads))
+    grads.push_back(std::move(t));
+  return grads;
+}
+
+// ----------------------------------------------------------------- updates of phi
+namespace {
+
+// Equal matrices: one [rows, cols] or [count, rows, cols] tensor, or a list of [rows, cols].
+struct Mats {
+  std::vector<at::Tensor> keep;   // contiguous copies
+  std::vector<void*> ptrs;
+  int64_t rows = 0, cols = 0;
+  int dtype = 0;
+  at::Device dev = at::kCPU;
+};
+
+Mats mats_of(at::TensorList x, const char* name, bool copy) {
+  Mats m;
+  TORCH_CHECK_VALUE(!x.empty(), name, " must not be an empty sequence");
+  const at::Tensor& t0 = x[0];
+  const int64_t dim = t0.dim();
+  TORCH_CHECK_VALUE(dim == 2 || (dim == 3 && x.size() == 1), name,
+                    " must be [rows, cols], [count, rows, cols] or a sequence of [rows, cols]");
+  m.rows = t0.size(dim - 2);
+  m.cols = t0.size(dim - 1);
+  m.dev = t0.device();
+  m.dtype = dtype_code(t0);
+  TORCH_CHECK_TYPE(m.dtype == MHC_F32 || m.dtype == MHC_BF16, name, " must be float32 or bfloat16, got ",
+                   t0.scalar_type());
+  TORCH_CHECK_VALUE(std::min(m.rows, m.cols) <= 80, name, " is ", str(m.rows), " x ", str(m.cols),
+                    ": the shorter side may have at most 80 rows");
+  m.ptrs.reserve(dim == 3 ? (size_t)t0.size(0) : x.size());
+  for (size_t i = 0; i < x.size(); ++i) {
+    at::Tensor t = x[i];
+    TORCH_CHECK_VALUE(t.sizes() == t0.sizes() && t.scalar_type() == t0.scalar_type() && t.device() == m.dev, name, "[",
+                      str((int64_t)i), "] is ", t.scalar_type(), " ", str(t.sizes()), " on ", t.device(), ", ", name,
+                      "[0] is ", t0.scalar_type(), " ", str(t0.sizes()), " on ", m.dev);
+    if (!t.is_contiguous()) {
+      TORCH_CHECK_VALUE(copy, name, "[", str((int64_t)i), "] must be contiguous");
+      t = t.contiguous();
+      m.keep.push_back(t);
+    }
+    char* p = static_cast<char*>(t.data_ptr());
+    if (dim == 2) {
+      m.ptrs.push_back(p);
+    } else {
+      for (int64_t j = 0; j < t.size(0); ++j) m.ptrs.push_back(p + j * m.rows * m.cols * t.element_size());
+    }
+  }
+  return m;
+}
+
+// Host doubles of the steps; count of triples.
+int32_t check_coeffs(at::ArrayRef<double> coeffs, double eps) {
+  TORCH_CHECK_VALUE(!coeffs.empty() && coeffs.size() % 3 == 0 && coeffs.size() <= 48,
+                    "coeffs must be 1 to 16 triples (a, b, c)");
+  TORCH_CHECK_VALUE(eps >= 1e-20, "eps must be at least 1e-20, got ", str(eps));
+  return (int32_t)(coeffs.size() / 3);
+}
+
+at::Tensor ortho_workspace(const Mats& m, size_t* nbytes) {
+  check_status(mhc_ortho_workspace_size((int64_t)m.ptrs.size(), (int32_t)m.rows, (int32_t)m.cols, nbytes),
+               "mhc_ortho_workspace_size");
+  return scratch(*nbytes, m.dev);
+}
+
+void check_sizes(const Mats& m) {
+  TORCH_CHECK_VALUE(std::max(m.rows, m.cols) <= (1 << 30), "a side of more than 2^30");
+}
+
+}  // namespace
+
+std::vector<at::Tensor> orthogonalize_cuda(at::TensorList g, at::ArrayRef<double> coeffs, double eps) {
+  mhc_ortho_args a{};
+  a.steps = check_coeffs(coeffs, eps);
+  c10::cuda::CUDAGuard guard(g.empty() ? at::Device(at::kCUDA, at::cuda::current_device()) : g[0].device());
+  const Mats m = mats_of(g, "g", true);
+  check_sizes(m);
+  const int64_t count = (int64_t)m.ptrs.size();
+  at::Tensor stack;
+  std::vector<at::Tensor> out;
+  if (g[0].dim() == 3 || g.size() == 1) {
+    stack = at::empty(g[0].sizes(), g[0].options());
+    out.push_back(stack);
+  } else {
+    stack = at::empty({count, m.rows, m.cols}, g[0].options());
+    out = stack.unbind(0);
+  }
+  std::vector<void*> dst(m.ptrs.size());
+  const int64_t step = m.rows * m.cols * (int64_t)stack.element_size();
+  for (int64_t i = 0; i < count; ++i) dst[i] = static_cast<char*>(stack.data_ptr()) + i * step;
+  const at::Tensor ws = ortho_workspace(m, &a.workspace_bytes);
+  a.in = m.ptrs.data();
+  a.out = dst.data();
+  a.count = count;
+  a.rows = (int32_t)m.rows;
+  a.cols = (int32_t)m.cols;
+  a.dtype = m.dtype;
+  a.coeffs = coeffs.data();
+  a.eps = eps;
+  a.workspace = ws.data_ptr();
+  check_status(mhc_orthogonalize(&a, at::cuda::getCurrentCUDAStream().stream()), "mhc::orthogonalize");
+  return out;
+}
+
+void muon_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList momenta, const OptTensor& lr_tensor,
+                    double lr, double momentum, bool nesterov, double weight_decay, double scale,
+                    at::ArrayRef<double> coeffs, double eps) {
+  mhc_muon_args a{};
+  a.steps = check_coeffs(coeffs, eps);
+  c10::cuda::CUDAGuard guard(params.empty() ? at::Device(at::kCUDA, at::cuda::current_device()) : params[0].device());
+  const Mats p = mats_of(params, "params", false), g = mats_of(grads, "grads", true),
+             m = mats_of(momenta, "momenta", false);
+  check_sizes(p);
+  TORCH_CHECK_VALUE(p.ptrs.size() == g.ptrs.size() && p.ptrs.size() == m.ptrs.size() && p.rows == g.rows &&
+                        p.rows == m.rows && p.cols == g.cols && p.cols == m.cols,
+                    "params, grads and momenta differ: ", str((int64_t)p.ptrs.size()), " of ", str(p.rows), " x ",
+                    str(p.cols), ", ", str((int64_t)g.ptrs.size()), " of ", str(g.rows), " x ", str(g.cols), ", ",
+                    str((int64_t)m.ptrs.size()), " of ", str(m.rows), " x ", str(m.cols));
+  TORCH_CHECK_VALUE(p.dev == g.dev && p.dev == m.dev, "params are on ", p.dev, ", grads on ", g.dev, ", momenta on ",
+                    m.dev);
+  TORCH_CHECK_TYPE(m.dtype == MHC_F32, "momenta must be float32, got ", momenta[0].scalar_type());
+  if (given(lr_tensor)) {
+    TORCH_CHECK_VALUE(lr_tensor->numel() == 1 && lr_tensor->scalar_type() == at::kFloat && lr_tensor->device() == p.dev,
+                      "lr must be a number or a one-element float32 tensor on ", p.dev);
+    a.lr_device = lr_tensor->data_ptr<float>();
+  }
+  const at::Tensor ws = ortho_workspace(p, &a.workspace_bytes);
+  a.params = p.ptrs.data();
+  a.grads = g.ptrs.data();
+  a.momenta = reinterpret_cast<float* const*>(m.ptrs.data());
+  a.count = (int64_t)p.ptrs.size();
+  a.rows = (int32_t)p.rows;
+  a.cols = (int32_t)p.cols;
+  a.param_dtype = p.dtype;
+  a.grad_dtype = g.dtype;
+  a.nesterov = nesterov ? 1 : 0;
+  a.coeffs = coeffs.data();
+  a.eps = eps;
+  a.momentum = (float)momentum;
+  a.weight_decay = (float)weight_decay;
+  a.scale = (float)scale;
+  a.lr = (float)lr;
+  a.workspace = ws.data_ptr();
+  check_status(mhc_muon_step(&a, at::cuda::getCurrentCUDAStream().stream()), "mhc::muon_step_");
+  // autograd has to see that these were written
+  for (const at::Tensor& t : params)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (const at::Tensor& t : momenta)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ----------------------------------------------------------------- Meta kernels (shapes only)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> mhc_fwd_meta(
     const at::Tensor& x, const at::Tensor& phi, const at::Tensor& alpha, const at::Tensor& bias, double, double) {
@@ -299,12 +698,72 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> mhc_bwd_m
           at::empty_symint({N}, f), at::empty_symint({n * D}, f)};
 }
 
+std::vector<at::Tensor> qk_norm_rope_meta(const at::Tensor& q, const at::Tensor& k, const OptTensor&,
+                                          const at::Tensor&, const OptTensor&, const OptTensor&, const OptTensor& v,
+                                          const OptTensor&, double, bool) {
+  std::vector<at::Tensor> out{at::empty_symint(q.sym_sizes(), q.options()),
+                              at::empty_symint(k.sym_sizes(), k.options())};
+  if (given(v)) out.push_back(at::empty_symint(v->sym_sizes(), v->options()));
+  return out;
+}
+
+std::vector<at::Tensor> qk_norm_rope_bwd_into_meta(const at::Tensor& q, const at::Tensor&, const OptTensor&,
+                                                   const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                   const OptTensor& q_weight, const OptTensor& k_weight,
+                                                   const OptTensor&, const OptTensor&, const OptTensor& row_scale,
+                                                   double, bool, bool weight_grads, bool row_scale_grad,
+                                                   at::TensorList) {
+  std::vector<at::Tensor> out;
+  const auto f = q.options().dtype(at::kFloat);
+  if (given(q_weight) && weight_grads) out.push_back(at::empty_symint({q.sym_size(3)}, f));
+  if (given(k_weight) && weight_grads) out.push_back(at::empty_symint({q.sym_size(3)}, f));
+  if (given(row_scale) && row_scale_grad) out.push_back(at::empty_symint({q.sym_size(0), q.sym_size(1)}, f));
+  return out;
+}
+
+std::vector<at::Tensor> qk_norm_rope_bwd_meta(const at::Tensor& q, const at::Tensor& k, const OptTensor& positions,
+                                              const at::Tensor& inv_freq, const at::Tensor& dq_out,
+                                              const at::Tensor& dk_out, const OptTensor& q_weight,
+                                              const OptTensor& k_weight, const OptTensor& v, const OptTensor& dv_out,
+                                              const OptTensor& row_scale, double eps, bool interleaved,
+                                              bool weight_grads, bool row_scale_grad) {
+  auto out = qk_norm_rope_meta(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps, interleaved);
+  for (auto& t : qk_norm_rope_bwd_into_meta(q, k, positions, inv_freq, dq_out, dk_out, q_weight, k_weight, v, dv_out,
+                                            row_scale, eps, interleaved, weight_grads, row_scale_grad, {}))
+    out.push_back(std::move(t));
+  return out;
+}
+
+std::vector<at::Tensor> orthogonalize_meta(at::TensorList g, at::ArrayRef<double>, double) {
+  std::vector<at::Tensor> out;
+  for (const at::Tensor& t : g) out.push_back(at::empty_symint(t.sym_sizes(), t.options()));
+  return out;
+}
+
+void muon_step_meta(at::TensorList, at::TensorList, at::TensorList, const OptTensor&, double, double, bool, double,
+                    double, at::ArrayRef<double>, double) {}
+
 TORCH_LIBRARY(mhc, m) {
   m.def("fwd(Tensor x, Tensor phi, Tensor alpha, Tensor bias, float norm_eps=1e-6, float hc_eps=1e-6) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("bwd(Tensor x, Tensor phi, Tensor alpha, Tensor inv_rms, Tensor h_mix, Tensor h_pre, Tensor h_post, "
         "Tensor dh_in, Tensor dh_post, Tensor dh_res, Tensor? gamma, float norm_eps=1e-6, float hc_eps=1e-6) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+  // q [B,S,Hq,d], k [B,S,Hk,d], v [B,S,Hv,d] -> q_out, k_out (, v_out)
+  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? positions, Tensor inv_freq, Tensor? q_weight, Tensor? k_weight, "
+        "Tensor? v, Tensor? row_scale, float eps, bool interleaved) -> Tensor[]");
+  // -> dq, dk (, dv) (, dq_weight) (, dk_weight) (, drow_scale): what is given and wanted
+  m.def("qk_norm_rope_bwd(Tensor q, Tensor k, Tensor? positions, Tensor inv_freq, Tensor dq_out, Tensor dk_out, "
+        "Tensor? q_weight, Tensor? k_weight, Tensor? v, Tensor? dv_out, Tensor? row_scale, float eps, "
+        "bool interleaved, bool weight_grads, bool row_scale_grad) -> Tensor[]");
+  // dq, dk (, dv) written into grad_out -> the rest
+  m.def("qk_norm_rope_bwd_into(Tensor q, Tensor k, Tensor? positions, Tensor inv_freq, Tensor dq_out, Tensor dk_out, "
+        "Tensor? q_weight, Tensor? k_weight, Tensor? v, Tensor? dv_out, Tensor? row_scale, float eps, "
+        "bool interleaved, bool weight_grads, bool row_scale_grad, Tensor(a!)[] grad_out) -> Tensor[]");
+  // equal matrices, or one stack of them; coeffs flat
+  m.def("orthogonalize(Tensor[] g, float[] coeffs, float eps) -> Tensor[]");
+  m.def("muon_step_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, Tensor? lr_tensor, float lr, "
+        "float momentum, bool nesterov, float weight_decay, float scale, float[] coeffs, float eps) -> ()");
   m.def("check_status() -> int");
   m.impl("check_status", &mhc_check_status);
 }
@@ -312,9 +771,26 @@ TORCH_LIBRARY(mhc, m) {
 TORCH_LIBRARY_IMPL(mhc, CUDA, m) {
   m.impl("fwd", &mhc_fwd_cuda);
   m.impl("bwd", &mhc_bwd_cuda);
+  m.impl("qk_norm_rope", &qk_norm_rope_cuda);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_cuda);
+  m.impl("qk_norm_rope_bwd_into", &qk_norm_rope_bwd_into_cuda);
+  m.impl("orthogonalize", &orthogonalize_cuda);
+  m.impl("muon_step_", &muon_step_cuda);
 }
 
 TORCH_LIBRARY_IMPL(mhc, Meta, m) {
   m.impl("fwd", &mhc_fwd_meta);
   m.impl("bwd", &mhc_bwd_meta);
+  m.impl("qk_norm_rope", &qk_norm_rope_meta);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_meta);
+  m.impl("qk_norm_rope_bwd_into", &qk_norm_rope_bwd_into_meta);
+  m.impl("orthogonalize", &orthogonalize_meta);
+  m.impl("muon_step_", &muon_step_meta);
+}
+
+// No gradient is recorded through these: the autograd Functions of the Python
+// layer are made of them, and the update writes leaves that require one.
+TORCH_LIBRARY_IMPL(mhc, Autograd, m) {
+  for (const char* op : {"qk_norm_rope", "qk_norm_rope_bwd", "qk_norm_rope_bwd_into", "orthogonalize", "muon_step_"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
 }

@@ -12,6 +12,11 @@ dgamma)``: the reference's ``mhc_backward_manual``
 (``src/backward/golden.py:10-96``), Triton call site
 ``src/backward/mhc_backward_triton.py:467-473``; ``gamma`` may be None.
 
+``qk_norm_rope`` / ``qk_norm_rope_bwd`` / ``qk_norm_rope_bwd_into``,
+``orthogonalize`` and ``muon_step_`` are the operators under
+``mhc_qk_norm_rope``, ``mhc_orthogonalize`` and ``mhc_muon_step``
+(``mhc_ops_b200.qkrope``, ``mhc_ops_b200.muon``), which document them.
+
 The operators run the same kernels as the ctypes API through the C ABI, on the
 current CUDA stream, and have Meta kernels, so FakeTensor tracing
 (``torch.compile``, ``torch.export``) sees them as single graph nodes.  CPU
@@ -30,7 +35,8 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "lib
 _lock = threading.Lock()
 _loaded = False
 
-__all__ = ["load", "fwd", "bwd", "check_status", "lib_path"]
+__all__ = ["load", "fwd", "bwd", "qk_norm_rope", "qk_norm_rope_bwd", "qk_norm_rope_bwd_into", "orthogonalize",
+           "muon_step_", "check_status", "lib_path"]
 
 
 def lib_path() -> str:
@@ -61,6 +67,23 @@ def bwd(x, phi, alpha, inv_rms, h_mix, h_pre, h_post, dh_in, dh_post, dh_res, ga
     load()
     return torch.ops.mhc.bwd(x, phi, alpha, inv_rms, h_mix, h_pre, h_post, dh_in, dh_post, dh_res, gamma,
                              norm_eps, hc_eps)
+
+
+def _bind(name):
+    """The operator's call without the overload lookup; looked up at the first call."""
+    def first(*args):
+        load()
+        op = getattr(torch.ops.mhc, name).default
+        globals()[name] = op
+        return op(*args)
+    return first
+
+
+qk_norm_rope = _bind("qk_norm_rope")
+qk_norm_rope_bwd = _bind("qk_norm_rope_bwd")
+qk_norm_rope_bwd_into = _bind("qk_norm_rope_bwd_into")
+orthogonalize = _bind("orthogonalize")
+muon_step_ = _bind("muon_step_")
 
 
 def check_status() -> None:

@@ -342,3 +342,12 @@ def test_refusals():
     with pytest.raises(ValueError, match="expanded"):
         back(grad_out=(torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device="cuda").expand(1, 4, 2, 64),
                        torch.empty_like(t["dk"])))
+
+
+def test_shape_errors_of_the_registered_operators_are_exceptions():
+    """Their messages name sizes; torch.ops.mhc.fwd's among them."""
+    from mhc_ops_b200 import ops
+    x = torch.zeros(1, 4, 2, 16, dtype=torch.bfloat16, device="cuda")
+    z = lambda *s: torch.zeros(*s, device="cuda")   # noqa: E731
+    with pytest.raises(RuntimeError, match=r"phi must be \[8, 32\], got \[8, 31\]"):
+        ops.fwd(x, z(8, 31), z(3), z(8))

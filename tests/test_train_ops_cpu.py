@@ -115,3 +115,21 @@ def test_data_parallel_update_takes_the_reduced_dphi():
     assert calls == ["wait", ((8, 8), 64.0, 0.1, {"weight_decay": 0.5})] and dp.pending is None
     with pytest.raises(ValueError, match="phi must be"):
         dp.muon_step(phi[:4], phi, 0.1)
+
+
+def test_meta_kernels_give_the_output_shapes():
+    """FakeTensor tracing sees each operator as one node with these outputs."""
+    from mhc_ops_b200 import ops
+    m = dict(device="meta", dtype=torch.bfloat16)
+    q, k, v = torch.empty(2, 5, 4, 16, **m), torch.empty(2, 5, 2, 16, **m), torch.empty(2, 5, 2, 16, **m)
+    f, w, s = torch.empty(8, device="meta"), torch.empty(16, device="meta"), torch.empty(2, 5, device="meta")
+    out = ops.qk_norm_rope(q, k, None, f, w, None, v, s, 1e-6, False)
+    assert [tuple(o.shape) for o in out] == [(2, 5, 4, 16), (2, 5, 2, 16), (2, 5, 2, 16)]
+    args = (q, k, None, f, q, k, w, w, v, v, s, 1e-6, False)
+    out = ops.qk_norm_rope_bwd(*args, True, True)
+    assert [tuple(o.shape) for o in out] == [(2, 5, 4, 16), (2, 5, 2, 16), (2, 5, 2, 16), (16,), (16,), (2, 5)]
+    assert [o.dtype for o in out[3:]] == [torch.float32] * 3
+    assert [tuple(o.shape) for o in ops.qk_norm_rope_bwd_into(*args, False, True, [q, k, v])] == [(2, 5)]
+    g = torch.empty(3, 8, 64, device="meta")
+    assert [tuple(o.shape) for o in ops.orthogonalize([g], [1.5, -0.5, 0.0], 1e-7)] == [(3, 8, 64)]
+    assert ops.muon_step_([g], [g], [g], None, 0.1, 0.9, True, 0.0, 1.0, [1.5, -0.5, 0.0], 1e-7) is None
