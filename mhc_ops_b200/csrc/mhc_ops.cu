@@ -1151,20 +1151,21 @@ int rope_check_view(const mhc_heads& h, const mhc_qk_args* a, int heads) {
 
 struct RopePlan {
   bool vec;
+  int gshift;   // vector kernels: logarithm of the lanes a head row takes
   int blocks;
   size_t smem;
 };
 
-// CTAs of the backward at most, so also rows of its weight-gradient partials.
-int rope_bwd_max_blocks(int sms) { return sms * 2; }
+// CTAs of the persistent kernels at most, so also rows of the backward's weight-gradient partials.
+int rope_max_blocks(int sms) { return sms * 2; }
 
 RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, int sms) {
   RopePlan r{};
-  p.q = rope_view(a->q);
-  p.k = rope_view(a->k);
-  p.v = rope_view(a->v);
-  p.wq = a->q_weight;
-  p.wk = a->k_weight;
+  p.x[0] = rope_view(a->q);
+  p.x[1] = rope_view(a->k);
+  p.x[2] = rope_view(a->v);
+  p.w[0] = a->q_weight;
+  p.w[1] = a->k_weight;
   p.inv_freq = a->inv_freq;
   p.pos = a->positions;
   p.pos64 = a->position_bytes == 8;
@@ -1173,44 +1174,68 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   p.row_scale = a->row_scale;
   p.T = a->batch * a->seq;
   p.S = (int)a->seq;
-  p.Hq = a->q_heads;
-  p.Hk = a->k_heads;
-  p.Hv = a->v.data ? a->v_heads : 0;
+  p.heads[0] = a->q_heads;
+  p.heads[1] = a->k_heads;
+  p.heads[2] = a->v.data ? a->v_heads : 0;
   p.d = a->d;
   p.rot = a->rot;
   p.eps = a->eps;
   r.vec = vec_views && a->d % 16 == 0 && a->d <= 512 && (a->interleaved || a->rot % 16 == 0);
-  const int H = p.Hq + p.Hk + p.Hv;
-  p.gshift = r.vec ? rope_log2(a->d / 16) : 5;
-  p.G = 1 << p.gshift;
-  const int hpw = 32 >> p.gshift;   // head rows a warp takes at a time, all of one side
-  const int groups = r.vec ? (p.Hq + hpw - 1) / hpw + (p.Hk + hpw - 1) / hpw + (p.Hv + hpw - 1) / hpw : H;
-  // Warps per token: one when the tokens alone fill the device (the angles are
-  // then computed once a token), more while there are few tokens.
-  p.parts = 1;
-  while (p.parts < rope::kWarps && p.parts < groups && p.T * p.parts < (int64_t)sms * rope::kWarps * 4) p.parts *= 2;
+  r.gshift = std::max(2, rope_log2(a->d / 16));   // heads of up to 64 elements share the 4-lane form
+  const int hpw = r.vec ? 32 >> r.gshift : 1;     // head rows a warp takes at a time, all of one side
+  int groups = 0;
+  for (int h : p.heads) groups += (h + hpw - 1) / hpw;
+  // Warps per token, the ones that need the fewest steps: rounds of the resident
+  // CTAs, each of a warp's share of the groups and about two groups' time for
+  // the token's angles and coefficients.  Every warp of a token has a group.
+  int64_t least = 0;
+  for (int parts = 1; parts <= rope::kWarps && (parts == 1 || parts <= groups); parts *= 2) {
+    const int64_t ctas = (p.T * parts + rope::kWarps - 1) / rope::kWarps;
+    const int64_t rounds = (ctas + rope_max_blocks(sms) - 1) / rope_max_blocks(sms);
+    const int64_t steps = rounds * ((groups + parts - 1) / parts + 2);
+    if (parts == 1 || steps < least) {
+      least = steps;
+      p.parts = parts;
+    }
+  }
   const int64_t tok_per_cta = rope::kWarps / p.parts;
   const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
-  r.blocks = (int)std::min<int64_t>(want, backward ? rope_bwd_max_blocks(sms) : (int64_t)sms * 16);
-  r.smem = (size_t)rope::kWarps * sizeof(float) * (r.vec ? (backward ? 1024 : 0) : p.rot + (backward ? 2 * p.d : 0));
+  r.blocks = (int)std::min<int64_t>(want, r.vec || backward ? rope_max_blocks(sms) : (int64_t)sms * 16);
+  r.smem = (size_t)rope::kWarps * sizeof(float) * (p.rot + (backward ? 2 * p.d : 0));   // the other kernels'
   return r;
+}
+
+template <class T, bool kInter, int kGS>
+int rope_launch_vec(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
+  // with its static arrays either ring is more than a kernel has without asking
+  if (backward) {
+    auto kernel = rope::bwd_vec_kernel<T, kInter, kGS>;
+    constexpr int sums = rope::kWarps * 1024 * (int)sizeof(float), ring = (int)rope::Ring<T, 2>::kBytes;
+    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring + sums));
+    kernel<<<r.blocks, rope::kThreads, ring + (p.dw_part ? sums : 0), s>>>(p);
+  } else {
+    auto kernel = rope::fwd_vec_kernel<T, kInter, kGS>;
+    constexpr int ring = (int)rope::Ring<T, 1>::kBytes;
+    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    kernel<<<r.blocks, rope::kThreads, ring, s>>>(p);
+  }
+  return after_launch();
 }
 
 template <class T, bool kInter>
 int rope_launch(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
-  if (backward) {
-    if (r.vec) {
-      // with its static arrays more than a kernel has without asking
-      MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_vec_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)r.smem));
-      rope::bwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, p.dw_part ? r.smem : 0, s>>>(p);
-    } else {
-      MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_any_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(rope::kWarps * 3 * rope::kMaxD * sizeof(float))));
-      rope::bwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
+  if (r.vec) {
+    switch (r.gshift) {
+      case 2: return rope_launch_vec<T, kInter, 2>(p, r, backward, s);
+      case 3: return rope_launch_vec<T, kInter, 3>(p, r, backward, s);
+      case 4: return rope_launch_vec<T, kInter, 4>(p, r, backward, s);
+      default: return rope_launch_vec<T, kInter, 5>(p, r, backward, s);
     }
-  } else if (r.vec) {
-    rope::fwd_vec_kernel<T, kInter><<<r.blocks, rope::kThreads, 0, s>>>(p);
+  }
+  if (backward) {
+    MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_any_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)(rope::kWarps * 3 * rope::kMaxD * sizeof(float))));
+    rope::bwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
   } else {
     rope::fwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
   }
@@ -1903,9 +1928,9 @@ int mhc_qk_norm_rope(const mhc_qk_args* a, void* stream) {
                    (!a->v.data || rope_view_vec(a->v_out, es));
   rope::Params p{};
   const RopePlan r = rope_plan(a, p, vec, false, sms);
-  p.oq = rope_view(a->q_out);
-  p.ok = rope_view(a->k_out);
-  p.ov = rope_view(a->v_out);
+  p.out[0] = rope_view(a->q_out);
+  p.out[1] = rope_view(a->k_out);
+  p.out[2] = rope_view(a->v_out);
 #ifdef MHC_DEBUG_BOUNDS
   if ((st = dbg_register_rope(a, nullptr, static_cast<cudaStream_t>(stream)))) return st;
 #endif
@@ -1917,7 +1942,7 @@ int mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t d, size_t* bytes
   if (tokens < 0 || d < 1 || d > rope::kMaxD) return MHC_ERR_BAD_SHAPE;
   int sms = 0;
   if (int st = current_sm_count(&sms)) return st;
-  *bytes = (size_t)std::min<int64_t>(std::max<int64_t>(tokens, 1), rope_bwd_max_blocks(sms)) * 2 * d * sizeof(float);
+  *bytes = (size_t)std::min<int64_t>(std::max<int64_t>(tokens, 1), rope_max_blocks(sms)) * 2 * d * sizeof(float);
   return MHC_OK;
 }
 
@@ -1961,12 +1986,12 @@ int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* b, void* stream) {
     if (b->workspace_bytes < (size_t)r.blocks * 2 * a->d * sizeof(float)) return MHC_ERR_WORKSPACE_TOO_SMALL;
     p.dw_part = static_cast<float*>(b->workspace);
   }
-  p.dq = rope_view(b->dq_out);
-  p.dk = rope_view(b->dk_out);
-  p.dv = rope_view(b->dv_out);
-  p.oq = rope_view(b->dq);
-  p.ok = rope_view(b->dk);
-  p.ov = rope_view(b->dv);
+  p.dy[0] = rope_view(b->dq_out);
+  p.dy[1] = rope_view(b->dk_out);
+  p.dy[2] = rope_view(b->dv_out);
+  p.out[0] = rope_view(b->dq);
+  p.out[1] = rope_view(b->dk);
+  p.out[2] = rope_view(b->dv);
   p.d_row_scale = b->d_row_scale;
 #ifdef MHC_DEBUG_BOUNDS
   if ((st = dbg_register_rope(a, b, s))) return st;

@@ -41,12 +41,12 @@ struct View {
   int64_t sb, ss, sh;
 };
 
+// Sides: 0 queries, 1 keys, 2 values (no head where there are none).
 struct Params {
-  View q, k, v;             // inputs (v.p NULL: no values)
-  View dq, dk, dv;          // backward: upstream gradients
-  View oq, ok, ov;          // outputs (forward) / input gradients (backward); written
-  const float* wq;          // [d] or NULL
-  const float* wk;
+  View x[3];                // inputs
+  View dy[3];               // backward: upstream gradients
+  View out[3];              // outputs (forward) / input gradients (backward); written
+  const float* w[2];        // [d] or NULL
   const float* inv_freq;    // [rot / 2]
   const void* pos;          // NULL: the token's index in its sequence
   const float* row_scale;   // [T] or NULL
@@ -56,9 +56,8 @@ struct Params {
   int64_t T;
   int S;
   int pos64;
-  int Hq, Hk, Hv;
+  int heads[3];
   int d, rot;
-  int G, gshift;            // vector kernels: lanes per head row, a power of two, and its logarithm
   int parts;                // warps that share a token's heads (1, 2, 4 or 8)
   float eps;
 };
@@ -189,10 +188,11 @@ __device__ __forceinline__ void apply_turn(const Turn& t, const float2 (&a)[4], 
   }
 }
 
-__device__ __forceinline__ float group_sum(float v, int G) {
+// Sum over the 2^kGS lanes of a head row.
+template <int kGS>
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    if (o < G) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 1; o < (1 << kGS); o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -201,44 +201,100 @@ __device__ __forceinline__ const T* row(const View& v, int b, int s, int h) {
   return static_cast<const T*>(v.p) + (b * v.sb + s * v.ss + h * v.sh);
 }
 
-// What a lane of the vector kernels works on: G lanes a head row with 16
-// elements each, 32 / G head rows of one token and one side (queries, keys or
-// values) at a time.
-struct Lane {
-  int G, u, hsub, hpw, oa, ob;
-  bool act;
-  int ng[3];   // head groups of each side
+// ------------------------------------------------------------ vector kernels
+// 2^kGS lanes take a head row, 16 elements each, so a warp has 32 >> kGS head
+// rows of one token and one side (queries, keys or values) at a time: a head
+// group.  Its groups are every parts-th of the list of its tokens' groups, queries
+// first, tokens `stride` apart.  Loads go through a ring in shared memory,
+// kDepth groups ahead and across tokens, that only the lane itself writes
+// (cp.async) and reads: depth without registers, no barrier.  With the next
+// group's loads in registers instead (one ahead) the forward took 91 us at
+// B=4, S=4096, 32+8+8 heads of 128, bf16, where a copy of the same rows takes 65.
+//
+// A cursor walks the groups with the lane's addresses in kN tensors.
+template <class T, int kGS, int kN>
+struct Cursor {
+  static constexpr int kHpw = 32 >> kGS;
+  const View* views[kN];   // [3] by side
+  const T* p[kN];
+  int64_t step[kN];
+  int64_t t, stride;
+  int part, hsub;
+  int side, left, h;       // left: groups of this side from here on, the other warps' among them
+
+  __device__ __forceinline__ bool more(const Params& P) const { return t < P.T; }
+  __device__ __forceinline__ bool in(const Params& P) const { return h < P.heads[side]; }
+  // to group `skip` from the start of `side`, of a later side or of the next token
+  __device__ __forceinline__ void enter(const Params& P, int skip) {
+    for (;;) {
+      if (side == 3) {
+        t += stride;
+        side = 0;
+        skip = part;
+      }
+      if (t >= P.T) return;
+      const int ng = (P.heads[side] + kHpw - 1) / kHpw;
+      if (skip < ng) {
+        left = ng - skip;
+        break;
+      }
+      skip -= ng;
+      ++side;
+    }
+    const int b = (int)((uint32_t)t / (uint32_t)P.S), s = (int)((uint32_t)t - (uint32_t)b * (uint32_t)P.S);
+    h = skip * kHpw + hsub;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      p[i] = row<T>(views[i][side], b, s, h);
+      step[i] = (int64_t)(P.parts * kHpw) * views[i][side].sh;
+    }
+  }
+  __device__ __forceinline__ void start(const Params& P, int64_t t0, int64_t stride_, int part_, int hsub_) {
+    t = t0;
+    stride = stride_;
+    part = part_;
+    hsub = hsub_;
+    side = 0;
+    enter(P, part);
+  }
+  __device__ __forceinline__ void advance(const Params& P) {
+    left -= P.parts;
+    if (left > 0) {
+      h += P.parts * kHpw;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) p[i] += step[i];
+    } else {
+      ++side;
+      enter(P, -left);
+    }
+  }
 };
-template <bool kInter>
-__device__ __forceinline__ Lane lane_of(const Params& P) {
-  Lane l;
-  const int lane = threadIdx.x & 31;
-  l.G = P.G;
-  l.u = lane & (P.G - 1);
-  l.hsub = lane >> P.gshift;
-  l.hpw = 32 >> P.gshift;
-  l.act = 16 * l.u < P.d;
-  unit_offsets<kInter>(l.u, P.rot, l.oa, l.ob);
-  l.ng[0] = (P.Hq + l.hpw - 1) / l.hpw;
-  l.ng[1] = (P.Hk + l.hpw - 1) / l.hpw;
-  l.ng[2] = (P.Hv + l.hpw - 1) / l.hpw;
-  return l;
+
+// 16 bytes to the lane's own slot, zeros when there is nothing to load.
+__device__ __forceinline__ void async16(uint4* dst, const void* src, bool in) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  const int bytes = in && MHC_CHK(src, 16) ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
 }
-// Head group g of the token's list: its side and this lane's head.
-__device__ __forceinline__ int group_side(const Params& P, const Lane& l, int g, int& h, bool& in) {
-  const int side = g < l.ng[0] ? 0 : g < l.ng[0] + l.ng[1] ? 1 : 2;
-  const int g0 = side == 0 ? 0 : side == 1 ? l.ng[0] : l.ng[0] + l.ng[1];
-  h = (g - g0) * l.hpw + l.hsub;
-  in = l.act && h < (side == 0 ? P.Hq : side == 1 ? P.Hk : P.Hv);
-  return side;
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
+// Groups in flight per warp and 16-byte words a lane has in each, for kN tensors.
+template <class T, int kN>
+struct Ring {
+  static constexpr int kWords = 2 * kN * Raw8<T>::kWords;
+  static constexpr int kDepth = kWords <= 2 ? 5 : kWords <= 4 ? 3 : 2;
+  static constexpr size_t kBytes = (size_t)kWarps * kDepth * kWords * 32 * 16;
+};
+
 // cos and sin of a token's rot / 2 angles into the warp's slots (ang[0] cos,
-// ang[1] sin; 1 and 0 up to the lanes' 8 per unit), each computed once a warp.
-__device__ __forceinline__ void token_angles(const Params& P, const Lane& l, int64_t pos, float (*ang)[256]) {
-  const int lane = threadIdx.x & 31;
+// ang[1] sin; 1 and 0 for the pairs that do not turn), each computed once a warp.
+__device__ __forceinline__ void token_angles(const Params& P, int64_t pos, float (*ang)[256]) {
   __syncwarp();   // the token before has been read
-  for (int i = lane; i < P.d / 2; i += 32) {
+  for (int i = threadIdx.x & 31; i < P.d / 2; i += 32) {
     float c = 1.f, s = 0.f;
     if (i < P.rot / 2) turn(pos, MHC_LDG(P.inv_freq + i), c, s);
     ang[0][i] = c;
@@ -246,303 +302,341 @@ __device__ __forceinline__ void token_angles(const Params& P, const Lane& l, int
   }
   __syncwarp();
 }
-__device__ __forceinline__ void unit_angles(const float (*ang)[256], const Lane& l, float (&cs)[8], float (&sn)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    cs[j] = l.act ? ang[0][8 * l.u + j] : 1.f;
-    sn[j] = l.act ? ang[1][8 * l.u + j] : 0.f;
-  }
-}
-
-// The unit's weights of a side from shared memory (ones without a weight).
-__device__ __forceinline__ void unit_weights(const float* sw, const Lane& l, float2 (&wa)[4], float2 (&wb)[4]) {
+// The unit's 8 values at [8 u] of a warp's angles.
+__device__ __forceinline__ void unit_angles(const float (*ang)[256], int u, float2 (&cs)[4], float2 (&sn)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    wa[j] = l.act ? *reinterpret_cast<const float2*>(sw + l.oa + 2 * j) : both(1.f);
-    wb[j] = l.act ? *reinterpret_cast<const float2*>(sw + l.ob + 2 * j) : both(1.f);
+    cs[j] = *reinterpret_cast<const float2*>(&ang[0][8 * u + 2 * j]);
+    sn[j] = *reinterpret_cast<const float2*>(&ang[1][8 * u + 2 * j]);
   }
 }
 __device__ __forceinline__ void load_weights(const Params& P, float (*sw)[512]) {
   for (int i = threadIdx.x; i < P.d; i += kThreads) {
-    sw[0][i] = P.wq ? MHC_LDG(P.wq + i) : 1.f;
-    sw[1][i] = P.wk ? MHC_LDG(P.wk + i) : 1.f;
+    sw[0][i] = P.w[0] ? MHC_LDG(P.w[0] + i) : 1.f;
+    sw[1][i] = P.w[1] ? MHC_LDG(P.w[1] + i) : 1.f;
   }
   __syncthreads();
 }
-
-// Forward, 16-byte vectors.  A warp takes a token's head groups (all of them,
-// or every parts-th), the next group's loads running during this one's
-// arithmetic.  The side's weights are folded into the turn's coefficients once
-// per token and side, so that a pair costs three packed instructions each way.
-template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3) fwd_vec_kernel(const Params P) {
-  __shared__ __align__(16) float sw[2][512];
-  __shared__ __align__(16) float angles[kWarps][2][256];
-  load_weights(P, sw);
-  const Lane l = lane_of<kInter>(P);
-  const int warp = threadIdx.x >> 5;
-  const int groups = l.ng[0] + l.ng[1] + l.ng[2];
-  const float inv_d = 1.f / (float)P.d;
-  const int part = warp & (P.parts - 1);
-  const int tok_per_cta = kWarps / P.parts;
-  for (int64_t t = (int64_t)blockIdx.x * tok_per_cta + warp / P.parts; t < P.T;
-       t += (int64_t)gridDim.x * tok_per_cta) {
-    const int b = (int)((uint32_t)t / (uint32_t)P.S), s = (int)((uint32_t)t - (uint32_t)b * (uint32_t)P.S);
-    auto fetch = [&](int g, Raw8<T>& ra, Raw8<T>& rb) {
-      int h;
-      bool in;
-      const int side = group_side(P, l, g, h, in);
-      ra.zero();
-      rb.zero();
-      if (g < groups && in) {
-        const T* src = row<T>(side == 0 ? P.q : side == 1 ? P.k : P.v, b, s, h);
-        ra.load(src + l.oa);
-        rb.load(src + l.ob);
-      }
-    };
-    Raw8<T> ra, rb;
-    fetch(part, ra, rb);
-    const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
-    token_angles(P, l, position(P, b, s), angles[warp]);
-    Turn tn;
-    int cur = -1;
-    for (int g = part; g < groups; g += P.parts) {
-      Raw8<T> na, nb;
-      fetch(g + P.parts, na, nb);
-      int h;
-      bool in;
-      const int side = group_side(P, l, g, h, in);
-      if (side != cur && side < 2) {   // the same for the whole warp
-        cur = side;
-        float2 wa[4], wb[4];
-        float cs[8], sn[8];
-        unit_weights(sw[side], l, wa, wb);
-        unit_angles(angles[warp], l, cs, sn);
+__device__ __forceinline__ void unit_weights(const float* sw, int oa, int ob, float2 (&wa)[4], float2 (&wb)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (kInter) {
-            tn.pa[j] = mul2(wa[j], both(cs[j]));
-            tn.qa[j] = mul2(swapped(wa[j]), make_float2(-sn[j], sn[j]));
-            tn.pb[j] = mul2(wb[j], both(cs[4 + j]));
-            tn.qb[j] = mul2(swapped(wb[j]), make_float2(-sn[4 + j], sn[4 + j]));
-          } else {
-            const float2 c2 = make_float2(cs[2 * j], cs[2 * j + 1]), s2 = make_float2(sn[2 * j], sn[2 * j + 1]);
-            tn.pa[j] = mul2(wa[j], c2);
-            tn.qa[j] = mul2(wb[j], make_float2(-s2.x, -s2.y));
-            tn.pb[j] = mul2(wb[j], c2);
-            tn.qb[j] = mul2(wa[j], s2);
-          }
-        }
-      }
-      float2 a[4], c[4], ya[4], yc[4];
-      ra.unpack(a);
-      rb.unpack(c);
-      float f = sc;
-      if (side < 2) {
-        float2 sq = mul2(a[0], a[0]);
-#pragma unroll
-        for (int j = 1; j < 4; ++j) sq = fma2(a[j], a[j], sq);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sq = fma2(c[j], c[j], sq);
-        const float ms = group_sum(sq.x + sq.y, l.G) * inv_d;
-        f = sc * __frsqrt_rn(fmaf(ms * sc, sc, P.eps));
-        apply_turn<kInter>(tn, a, c, ya, yc);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ya[j] = a[j], yc[j] = c[j];
-      }
-      if (in) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          ya[j] = mul2(ya[j], both(f));
-          yc[j] = mul2(yc[j], both(f));
-        }
-        T* dst = const_cast<T*>(row<T>(side == 0 ? P.oq : side == 1 ? P.ok : P.ov, b, s, h));
-        store8(dst + l.oa, ya);
-        store8(dst + l.ob, yc);
-      }
-      ra = na;
-      rb = nb;
-    }
+  for (int j = 0; j < 4; ++j) {
+    wa[j] = *reinterpret_cast<const float2*>(sw + oa + 2 * j);
+    wb[j] = *reinterpret_cast<const float2*>(sw + ob + 2 * j);
   }
 }
 
-// Backward, 16-byte vectors, the forward's split.  Each lane keeps the weight
-// gradients of its 16 elements: in registers over a side's head groups, in its
-// own shared-memory slots over tokens.  The CTA's warps are added in warp order
-// and the CTA's row written for the finalize kernel, so repeated calls give the
-// same bits.
-template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const Params P) {
+// Lanes beyond a row of d elements work on unit 0's coefficients and on zeros.
+template <bool kInter, int kGS>
+__device__ __forceinline__ bool lane_unit(const Params& P, int lane, int& u, int& oa, int& ob) {
+  u = lane & ((1 << kGS) - 1);
+  const bool act = 16 * u < P.d;
+  if (!act) u = 0;
+  unit_offsets<kInter>(u, P.rot, oa, ob);
+  return act;
+}
+
+// Forward.  The side's weights are folded into the turn's coefficients once per
+// token and side, so that a pair costs three packed instructions each way.
+template <class T, bool kInter, int kGS>
+__global__ void __launch_bounds__(kThreads, 2) fwd_vec_kernel(const __grid_constant__ Params P) {
+  __shared__ __align__(16) float sw[2][512];
+  __shared__ __align__(16) float angles[kWarps][2][256];
+  extern __shared__ __align__(16) uint4 ring[];   // [kWarps][kDepth][kWords][32]
+  using R = Ring<T, 1>;
+  constexpr int kW = Raw8<T>::kWords;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int u, oa, ob;
+  const bool act = lane_unit<kInter, kGS>(P, lane, u, oa, ob);
+  uint4* slots = ring + (warp * R::kDepth * R::kWords) * 32 + lane;
+  const float inv_d = 1.f / (float)P.d;
+  const int tok_per_cta = kWarps / P.parts, part = warp & (P.parts - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * tok_per_cta + warp / P.parts, stride = (int64_t)gridDim.x * tok_per_cta;
+  Cursor<T, kGS, 1> f, c;
+  f.views[0] = P.x;
+  c.views[0] = P.out;
+  f.start(P, t0, stride, part, lane >> kGS);
+  c.start(P, t0, stride, part, lane >> kGS);
+  auto issue = [&](int slot) {
+    uint4* dst = slots + slot * R::kWords * 32;
+    if (f.more(P)) {
+      const bool in = act && f.in(P);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        async16(dst + i * 32, reinterpret_cast<const uint4*>(f.p[0] + oa) + i, in);
+        async16(dst + (kW + i) * 32, reinterpret_cast<const uint4*>(f.p[0] + ob) + i, in);
+      }
+      f.advance(P);
+    }
+    async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < R::kDepth; ++i) issue(i);
+  load_weights(P, sw);
+  int64_t token = -1;
+  int cur = -1, slot = 0;
+  float sc = 1.f;
+  Turn tn;
+  while (c.more(P)) {
+    const int side = c.side;
+    if (c.t != token) {
+      token = c.t;
+      cur = -1;
+      const int b = (int)((uint32_t)token / (uint32_t)P.S), s = (int)((uint32_t)token - (uint32_t)b * (uint32_t)P.S);
+      if (P.row_scale) sc = MHC_LDG(P.row_scale + token);
+      token_angles(P, position(P, b, s), angles[warp]);
+    }
+    if (side != cur && side < 2) {   // the same for the whole warp
+      cur = side;
+      float2 wa[4], wb[4], cs[4], sn[4];
+      unit_weights(sw[side], oa, ob, wa, wb);
+      unit_angles(angles[warp], u, cs, sn);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kInter) {
+          const float c0 = j & 1 ? cs[j / 2].y : cs[j / 2].x, s0 = j & 1 ? sn[j / 2].y : sn[j / 2].x;
+          const float c1 = j & 1 ? cs[2 + j / 2].y : cs[2 + j / 2].x, s1 = j & 1 ? sn[2 + j / 2].y : sn[2 + j / 2].x;
+          tn.pa[j] = mul2(wa[j], both(c0));
+          tn.qa[j] = mul2(swapped(wa[j]), make_float2(-s0, s0));
+          tn.pb[j] = mul2(wb[j], both(c1));
+          tn.qb[j] = mul2(swapped(wb[j]), make_float2(-s1, s1));
+        } else {
+          tn.pa[j] = mul2(wa[j], cs[j]);
+          tn.qa[j] = mul2(wb[j], make_float2(-sn[j].x, -sn[j].y));
+          tn.pb[j] = mul2(wb[j], cs[j]);
+          tn.qb[j] = mul2(wa[j], sn[j]);
+        }
+      }
+    }
+    async_wait<R::kDepth - 1>();
+    const uint4* src = slots + slot * R::kWords * 32;
+    Raw8<T> ra, rb;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) ra.w[i] = src[i * 32], rb.w[i] = src[(kW + i) * 32];
+    float2 x0[4], x1[4], y0[4], y1[4];
+    ra.unpack(x0);
+    rb.unpack(x1);
+    float fct = sc;
+    if (side < 2) {
+      float2 sq = mul2(x0[0], x0[0]), sq1 = mul2(x1[0], x1[0]);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) {
+        sq = fma2(x0[j], x0[j], sq);
+        sq1 = fma2(x1[j], x1[j], sq1);
+      }
+      const float ms = group_sum<kGS>((sq.x + sq.y) + (sq1.x + sq1.y)) * inv_d;
+      fct = sc * rsqrtf(fmaf(ms * sc, sc, P.eps));
+      apply_turn<kInter>(tn, x0, x1, y0, y1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y0[j] = x0[j], y1[j] = x1[j];
+    }
+    issue(slot);
+    slot = slot + 1 == R::kDepth ? 0 : slot + 1;
+    if (act && c.in(P)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y0[j] = mul2(y0[j], both(fct));
+        y1[j] = mul2(y1[j], both(fct));
+      }
+      T* dst = const_cast<T*>(c.p[0]);
+      store8(dst + oa, y0);
+      store8(dst + ob, y1);
+    }
+    c.advance(P);
+  }
+}
+
+// Backward.  Each lane keeps the weight gradients of its 16 elements: in
+// registers over a side's head groups, in its own shared-memory slots over
+// tokens.  The CTA's warps are added in warp order and the CTA's row written for
+// the finalize kernel, so repeated calls give the same bits.
+template <class T, bool kInter, int kGS>
+__global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const __grid_constant__ Params P) {
   __shared__ __align__(16) float sw[2][512];
   __shared__ __align__(16) float angles[kWarps][2][256];
   __shared__ float sds[kWarps];
-  extern __shared__ __align__(16) float dyn[];   // [kWarps][2][16][32] weight gradients, with dw_part only
-  load_weights(P, sw);
-  const Lane l = lane_of<kInter>(P);
+  extern __shared__ __align__(16) uint4 ring[];   // [kWarps][kDepth][kWords][32], then the gradients
+  using R = Ring<T, 2>;
+  constexpr int kW = Raw8<T>::kWords;
+  float* dyn = reinterpret_cast<float*>(ring + R::kBytes / 16);   // [kWarps][2][16][32], with dw_part only
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int u, oa, ob;
+  const bool act = lane_unit<kInter, kGS>(P, lane, u, oa, ob);
+  uint4* slots = ring + (warp * R::kDepth * R::kWords) * 32 + lane;
   float* gacc = dyn + warp * 1024 + lane;
+  const float inv_d = 1.f / (float)P.d;
+  const int tok_per_cta = kWarps / P.parts, part = warp & (P.parts - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * tok_per_cta + warp / P.parts, stride = (int64_t)gridDim.x * tok_per_cta;
+  Cursor<T, kGS, 2> f;
+  Cursor<T, kGS, 1> c;
+  f.views[0] = P.x;
+  f.views[1] = P.dy;
+  c.views[0] = P.out;
+  f.start(P, t0, stride, part, lane >> kGS);
+  c.start(P, t0, stride, part, lane >> kGS);
+  auto issue = [&](int slot) {
+    uint4* dst = slots + slot * R::kWords * 32;
+    if (f.more(P)) {
+      const bool in = act && f.in(P);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+          async16(dst + (2 * n * kW + i) * 32, reinterpret_cast<const uint4*>(f.p[n] + oa) + i, in);
+          async16(dst + ((2 * n + 1) * kW + i) * 32, reinterpret_cast<const uint4*>(f.p[n] + ob) + i, in);
+        }
+      f.advance(P);
+    }
+    async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < R::kDepth; ++i) issue(i);
   if (P.dw_part)
     for (int i = 0; i < 32; ++i) gacc[i * 32] = 0.f;
-  const int groups = l.ng[0] + l.ng[1] + l.ng[2];
-  const float inv_d = 1.f / (float)P.d;
-  const int part = warp & (P.parts - 1);
-  const int tok_per_cta = kWarps / P.parts;
-  // every warp makes the same number of rounds: the row factor's sum over a
-  // token's warps needs a barrier per round
-  for (int64_t t0 = (int64_t)blockIdx.x * tok_per_cta; t0 < P.T; t0 += (int64_t)gridDim.x * tok_per_cta) {
-    const int64_t t = t0 + warp / P.parts;
-    float ds = 0.f;
-    if (t < P.T) {
-      const int b = (int)((uint32_t)t / (uint32_t)P.S), s = (int)((uint32_t)t - (uint32_t)b * (uint32_t)P.S);
-      auto fetch = [&](int g, Raw8<T>& xa, Raw8<T>& xb, Raw8<T>& ya, Raw8<T>& yb) {
-        int h;
-        bool in;
-        const int side = group_side(P, l, g, h, in);
-        xa.zero();
-        xb.zero();
-        ya.zero();
-        yb.zero();
-        if (g < groups && in) {
-          const T* x = row<T>(side == 0 ? P.q : side == 1 ? P.k : P.v, b, s, h);
-          const T* y = row<T>(side == 0 ? P.dq : side == 1 ? P.dk : P.dv, b, s, h);
-          xa.load(x + l.oa);
-          xb.load(x + l.ob);
-          ya.load(y + l.oa);
-          yb.load(y + l.ob);
-        }
-      };
-      Raw8<T> xa, xb, ya, yb;
-      fetch(part, xa, xb, ya, yb);
-      const float sc = P.row_scale ? MHC_LDG(P.row_scale + t) : 1.f;
-      float cs[8], sn[8];
-      token_angles(P, l, position(P, b, s), angles[warp]);
-      unit_angles(angles[warp], l, cs, sn);
-      float2 wa[4], wb[4], ga[4], gb[4];
-      int cur = -1;
-      auto flush = [&]() {   // the side's sums into the lane's slots
-        if (P.dw_part && cur >= 0) {
-          float* g = gacc + cur * 512;
+  load_weights(P, sw);
+  float2 cs[4], sn[4], wa[4], wb[4], ga[4], gb[4];
+  int64_t token = -1;
+  int cur = -1, slot = 0;
+  float sc = 1.f, ds = 0.f;
+  auto flush = [&]() {   // the side's sums into the lane's slots
+    if (P.dw_part && cur >= 0) {
+      float* g = gacc + cur * 512;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            g[(2 * j) * 32] += ga[j].x;
-            g[(2 * j + 1) * 32] += ga[j].y;
-            g[(8 + 2 * j) * 32] += gb[j].x;
-            g[(8 + 2 * j + 1) * 32] += gb[j].y;
-          }
-        }
-      };
-      for (int g = part; g < groups; g += P.parts) {
-        Raw8<T> nxa, nxb, nya, nyb;
-        fetch(g + P.parts, nxa, nxb, nya, nyb);
-        int h;
-        bool in;
-        const int side = group_side(P, l, g, h, in);
-        float2 x0[4], x1[4], y0[4], y1[4], o0[4], o1[4];
-        xa.unpack(x0);
-        xb.unpack(x1);
-        ya.unpack(y0);
-        yb.unpack(y1);
-        if (side < 2) {
-          if (side != cur) {
-            flush();
-            cur = side;
-            unit_weights(sw[side], l, wa, wb);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ga[j] = gb[j] = both(0.f);
-          }
-          float2 d0[4], d1[4];   // da = Rot^T dy
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (kInter) {
-              d0[j] = fma2(swapped(y0[j]), make_float2(sn[j], -sn[j]), mul2(y0[j], both(cs[j])));
-              d1[j] = fma2(swapped(y1[j]), make_float2(sn[4 + j], -sn[4 + j]), mul2(y1[j], both(cs[4 + j])));
-            } else {
-              const float2 c2 = make_float2(cs[2 * j], cs[2 * j + 1]), s2 = make_float2(sn[2 * j], sn[2 * j + 1]);
-              d0[j] = fma2(y1[j], s2, mul2(y0[j], c2));
-              d1[j] = fma2(y0[j], make_float2(-s2.x, -s2.y), mul2(y1[j], c2));
-            }
-          }
-          float2 sq = both(0.f), dt = both(0.f);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            sq = fma2(x0[j], x0[j], sq);
-            sq = fma2(x1[j], x1[j], sq);
-            y0[j] = mul2(d0[j], x0[j]);   // da x
-            y1[j] = mul2(d1[j], x1[j]);
-            dt = fma2(y0[j], wa[j], dt);
-            dt = fma2(y1[j], wb[j], dt);
-          }
-          const float ms = group_sum(sq.x + sq.y, l.G) * inv_d;
-          const float dot = group_sum(dt.x + dt.y, l.G);   // sum(dn x)
-          // a lane without a row adds nothing, whatever eps
-          const float r = in ? __frsqrt_rn(fmaf(ms * sc, sc, P.eps)) : 0.f;
-          const float sr = sc * r;
-          const float m2 = -sr * (sr * dot * inv_d);   // -s r m
-          if (l.u == 0) ds += P.eps * r * r * r * dot;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            ga[j] = fma2(y0[j], both(sr), ga[j]);
-            gb[j] = fma2(y1[j], both(sr), gb[j]);
-            o0[j] = mul2(both(sr), fma2(both(m2), x0[j], mul2(d0[j], wa[j])));
-            o1[j] = mul2(both(sr), fma2(both(m2), x1[j], mul2(d1[j], wb[j])));
-          }
-        } else {
-          float2 dt = both(0.f);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            dt = fma2(x0[j], y0[j], dt);
-            dt = fma2(x1[j], y1[j], dt);
-            o0[j] = mul2(both(sc), y0[j]);
-            o1[j] = mul2(both(sc), y1[j]);
-          }
-          ds += dt.x + dt.y;
-        }
-        if (in) {
-          T* dst = const_cast<T*>(row<T>(side == 0 ? P.oq : side == 1 ? P.ok : P.ov, b, s, h));
-          store8(dst + l.oa, o0);
-          store8(dst + l.ob, o1);
-        }
-        xa = nxa;
-        xb = nxb;
-        ya = nya;
-        yb = nyb;
+      for (int j = 0; j < 4; ++j) {
+        g[(2 * j) * 32] += ga[j].x;
+        g[(2 * j + 1) * 32] += ga[j].y;
+        g[(8 + 2 * j) * 32] += gb[j].x;
+        g[(8 + 2 * j + 1) * 32] += gb[j].y;
       }
-      flush();
     }
-    if (P.d_row_scale) {
-      ds = warp_sum(ds);
-      if (P.parts == 1) {
-        if (lane == 0 && t < P.T) MHC_ST(P.d_row_scale + t, ds);
-      } else {
-        if (lane == 0) sds[warp] = ds;
-        __syncthreads();
-        if (part == 0 && lane == 0 && t < P.T) {
-          float sum = 0.f;
-          for (int i = 0; i < P.parts; ++i) sum += sds[warp + i];
-          MHC_ST(P.d_row_scale + t, sum);
+  };
+  while (c.more(P)) {
+    const int side = c.side;
+    if (c.t != token) {
+      token = c.t;
+      cur = -1;
+      ds = 0.f;
+      const int b = (int)((uint32_t)token / (uint32_t)P.S), s = (int)((uint32_t)token - (uint32_t)b * (uint32_t)P.S);
+      if (P.row_scale) sc = MHC_LDG(P.row_scale + token);
+      token_angles(P, position(P, b, s), angles[warp]);
+      unit_angles(angles[warp], u, cs, sn);
+    }
+    if (side != cur && side < 2) {
+      flush();
+      cur = side;
+      unit_weights(sw[side], oa, ob, wa, wb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ga[j] = gb[j] = both(0.f);
+    }
+    async_wait<R::kDepth - 1>();
+    const uint4* src = slots + slot * R::kWords * 32;
+    Raw8<T> ra, rb;
+    float2 x0[4], x1[4], y0[4], y1[4];
+#pragma unroll
+    for (int i = 0; i < kW; ++i) ra.w[i] = src[i * 32], rb.w[i] = src[(kW + i) * 32];
+    ra.unpack(x0);
+    rb.unpack(x1);
+#pragma unroll
+    for (int i = 0; i < kW; ++i) ra.w[i] = src[(2 * kW + i) * 32], rb.w[i] = src[(3 * kW + i) * 32];
+    ra.unpack(y0);
+    rb.unpack(y1);
+    const bool in = act && c.in(P);
+    if (side < 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {   // da = Rot^T dy, in place
+        const float2 g0 = y0[j], g1 = y1[j];
+        if constexpr (kInter) {
+          const float c0 = j & 1 ? cs[j / 2].y : cs[j / 2].x, s0 = j & 1 ? sn[j / 2].y : sn[j / 2].x;
+          const float c1 = j & 1 ? cs[2 + j / 2].y : cs[2 + j / 2].x, s1 = j & 1 ? sn[2 + j / 2].y : sn[2 + j / 2].x;
+          y0[j] = fma2(swapped(g0), make_float2(s0, -s0), mul2(g0, both(c0)));
+          y1[j] = fma2(swapped(g1), make_float2(s1, -s1), mul2(g1, both(c1)));
+        } else {
+          y0[j] = fma2(g1, sn[j], mul2(g0, cs[j]));
+          y1[j] = fma2(g0, make_float2(-sn[j].x, -sn[j].y), mul2(g1, cs[j]));
         }
-        __syncthreads();
+      }
+      float2 sq = both(0.f), dt = both(0.f), sq1 = both(0.f), dt1 = both(0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sq = fma2(x0[j], x0[j], sq);
+        sq1 = fma2(x1[j], x1[j], sq1);
+        dt = fma2(mul2(y0[j], x0[j]), wa[j], dt);
+        dt1 = fma2(mul2(y1[j], x1[j]), wb[j], dt1);
+      }
+      const float ms = group_sum<kGS>((sq.x + sq.y) + (sq1.x + sq1.y)) * inv_d;
+      const float dot = group_sum<kGS>((dt.x + dt.y) + (dt1.x + dt1.y));   // sum(dn x)
+      issue(slot);
+      // a lane without a row adds nothing, whatever eps
+      const float r = in ? rsqrtf(fmaf(ms * sc, sc, P.eps)) : 0.f;
+      const float sr = sc * r;
+      const float m2 = -sr * (sr * dot * inv_d);   // -s r m
+      if ((lane & ((1 << kGS) - 1)) == 0) ds += P.eps * r * r * r * dot;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 n0 = mul2(both(sr), x0[j]), n1 = mul2(both(sr), x1[j]);
+        ga[j] = fma2(y0[j], n0, ga[j]);
+        gb[j] = fma2(y1[j], n1, gb[j]);
+        y0[j] = mul2(both(sr), fma2(both(m2), x0[j], mul2(y0[j], wa[j])));
+        y1[j] = mul2(both(sr), fma2(both(m2), x1[j], mul2(y1[j], wb[j])));
+      }
+    } else {
+      float2 dt = both(0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dt = fma2(x0[j], y0[j], dt);
+        dt = fma2(x1[j], y1[j], dt);
+        y0[j] = mul2(both(sc), y0[j]);
+        y1[j] = mul2(both(sc), y1[j]);
+      }
+      ds += dt.x + dt.y;
+      issue(slot);
+    }
+    slot = slot + 1 == R::kDepth ? 0 : slot + 1;
+    if (in) {
+      T* dst = const_cast<T*>(c.p[0]);
+      store8(dst + oa, y0);
+      store8(dst + ob, y1);
+    }
+    c.advance(P);
+    if (c.t != token) {   // the token's last group of this warp
+      flush();
+      if (P.d_row_scale) {
+        ds = warp_sum(ds);
+        if (P.parts == 1) {
+          if (lane == 0) MHC_ST(P.d_row_scale + token, ds);
+        } else {
+          // the token's warps walk the same tokens: one named barrier for each set of them
+          const int id = 1 + warp / P.parts, count = P.parts * 32;
+          if (lane == 0) sds[warp] = ds;
+          asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+          if (part == 0 && lane == 0) {
+            float sum = 0.f;
+            for (int i = 0; i < P.parts; ++i) sum += sds[warp + i];
+            MHC_ST(P.d_row_scale + token, sum);
+          }
+          asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
+        }
       }
     }
   }
+  async_wait<0>();
   if (P.dw_part) {
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * P.d; i += kThreads) {
       const int side = i >= P.d, col = i - side * P.d;
       // the unit and the place in it that hold this column
-      int u, e;
+      int unit, e;
       if (!kInter && col < P.rot) {
-        const int half = P.rot / 2, c = col < half ? col : col - half;
-        u = c / 8;
-        e = (col < half ? 0 : 8) + c % 8;
+        const int half = P.rot / 2, cc = col < half ? col : col - half;
+        unit = cc / 8;
+        e = (col < half ? 0 : 8) + cc % 8;
       } else {
-        u = col / 16;
+        unit = col / 16;
         e = col % 16;
       }
       float sum = 0.f;
       for (int w = 0; w < kWarps; ++w)
-        for (int k = 0; k < l.hpw; ++k) sum += dyn[w * 1024 + side * 512 + e * 32 + (k << P.gshift) + u];
+        for (int k = 0; k < (32 >> kGS); ++k) sum += dyn[w * 1024 + side * 512 + e * 32 + (k << kGS) + unit];
       MHC_ST(P.dw_part + (int64_t)blockIdx.x * 2 * P.d + i, sum);
     }
   }
@@ -552,14 +646,19 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const Params P) {
 // l, l + 32, ... and the passing elements likewise.  Dynamic shared memory per
 // warp: the token's cos and sin [rot/2] and, in the backward, the weight
 // gradients [2][d] of the warp (a lane only ever touches its own columns).
+__device__ __forceinline__ void head_side(const Params& P, int h, int& side, int& hh) {
+  side = h < P.heads[0] ? 0 : h < P.heads[0] + P.heads[1] ? 1 : 2;
+  hh = h - (side > 0 ? P.heads[0] : 0) - (side > 1 ? P.heads[1] : 0);
+}
+
 template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads) fwd_any_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads) fwd_any_kernel(const __grid_constant__ Params P) {
   extern __shared__ float dyn[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = P.rot / 2;
   float* cs = dyn + warp * P.rot;
   float* sn = cs + half;
-  const int H = P.Hq + P.Hk + P.Hv, Hqk = P.Hq + P.Hk;
+  const int H = P.heads[0] + P.heads[1] + P.heads[2];
   const float inv_d = 1.f / (float)P.d;
   const int part = warp & (P.parts - 1);
   const int tok_per_cta = kWarps / P.parts;
@@ -570,11 +669,11 @@ __global__ void __launch_bounds__(kThreads) fwd_any_kernel(const Params P) {
     const int64_t pos = position(P, b, s);
     for (int i = lane; i < half; i += 32) turn(pos, MHC_LDG(P.inv_freq + i), cs[i], sn[i]);   // own lane's slots
     for (int h = part; h < H; h += P.parts) {
-      const bool isq = h < P.Hq, isk = !isq && h < Hqk;
-      const int hh = isq ? h : isk ? h - P.Hq : h - Hqk;
-      const T* x = row<T>(isq ? P.q : isk ? P.k : P.v, b, s, hh);
-      T* y = const_cast<T*>(row<T>(isq ? P.oq : isk ? P.ok : P.ov, b, s, hh));
-      if (!isq && !isk) {
+      int side, hh;
+      head_side(P, h, side, hh);
+      const T* x = row<T>(P.x[side], b, s, hh);
+      T* y = const_cast<T*>(row<T>(P.out[side], b, s, hh));
+      if (side == 2) {
         for (int i = lane; i < P.d; i += 32) store1(y + i, load1(x + i) * sc);
         continue;
       }
@@ -584,8 +683,8 @@ __global__ void __launch_bounds__(kThreads) fwd_any_kernel(const Params P) {
         sq = fmaf(z, z, sq);
       }
       sq = warp_sum(sq);
-      const float r = __frsqrt_rn(fmaf(sq, inv_d, P.eps));
-      const float* w = isq ? P.wq : P.wk;
+      const float r = rsqrtf(fmaf(sq, inv_d, P.eps));
+      const float* w = P.w[side];
       for (int i = lane; i < half; i += 32) {
         const int ia = kInter ? 2 * i : i, ib = kInter ? 2 * i + 1 : i + half;
         const float a = load1(x + ia) * sc * r * (w ? MHC_LDG(w + ia) : 1.f);
@@ -600,7 +699,7 @@ __global__ void __launch_bounds__(kThreads) fwd_any_kernel(const Params P) {
 }
 
 template <class T, bool kInter>
-__global__ void __launch_bounds__(kThreads) bwd_any_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads) bwd_any_kernel(const __grid_constant__ Params P) {
   extern __shared__ float dyn[];
   __shared__ float sds[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -610,7 +709,7 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const Params P) {
   float* gw = dyn + warp * (P.rot + 2 * P.d) + P.rot;   // [2][d]
   for (int i = lane; i < 2 * P.d; i += 32) gw[i] = 0.f;
   __syncwarp();
-  const int H = P.Hq + P.Hk + P.Hv, Hqk = P.Hq + P.Hk;
+  const int H = P.heads[0] + P.heads[1] + P.heads[2];
   const float inv_d = 1.f / (float)P.d;
   const int part = warp & (P.parts - 1);
   const int tok_per_cta = kWarps / P.parts;
@@ -623,12 +722,12 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const Params P) {
       const int64_t pos = position(P, b, s);
       for (int i = lane; i < half; i += 32) turn(pos, MHC_LDG(P.inv_freq + i), cs[i], sn[i]);
       for (int h = part; h < H; h += P.parts) {
-        const bool isq = h < P.Hq, isk = !isq && h < Hqk;
-        const int hh = isq ? h : isk ? h - P.Hq : h - Hqk;
-        const T* x = row<T>(isq ? P.q : isk ? P.k : P.v, b, s, hh);
-        const T* dy = row<T>(isq ? P.dq : isk ? P.dk : P.dv, b, s, hh);
-        T* dx = const_cast<T*>(row<T>(isq ? P.oq : isk ? P.ok : P.ov, b, s, hh));
-        if (!isq && !isk) {
+        int side, hh;
+        head_side(P, h, side, hh);
+        const T* x = row<T>(P.x[side], b, s, hh);
+        const T* dy = row<T>(P.dy[side], b, s, hh);
+        T* dx = const_cast<T*>(row<T>(P.out[side], b, s, hh));
+        if (side == 2) {
           for (int i = lane; i < P.d; i += 32) {
             const float g = load1(dy + i);
             ds = fmaf(load1(x + i), g, ds);
@@ -636,8 +735,8 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const Params P) {
           }
           continue;
         }
-        const float* w = isq ? P.wq : P.wk;
-        float* g = gw + (isq ? 0 : P.d);
+        const float* w = P.w[side];
+        float* g = gw + side * P.d;
         float sq = 0.f, dot = 0.f;
         for (int i = lane; i < P.d; i += 32) {
           const float z = load1(x + i) * sc;
@@ -655,7 +754,7 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const Params P) {
           dot = fmaf(load1(dy + i) * (w ? MHC_LDG(w + i) : 1.f), load1(x + i), dot);
         sq = warp_sum(sq);
         dot = warp_sum(dot);
-        const float r = __frsqrt_rn(fmaf(sq, inv_d, P.eps));
+        const float r = rsqrtf(fmaf(sq, inv_d, P.eps));
         const float sr = sc * r;
         const float m = sr * dot * inv_d;
         if (lane == 0) ds += P.eps * r * r * r * dot;
