@@ -1255,11 +1255,13 @@ int rope_dispatch(const mhc_qk_args* a, const rope::Params& p, const RopePlan& r
 
 // ------------------------------------------------------- updates of phi
 struct OrthoPlan {
-  int R, C, NB, slices, chunks_per_slice, mats;   // mats: matrices of one launch
+  int R, C, NB, chunks, gram_ctas, segments, apply_ctas, mats;   // mats: matrices of one launch
   int64_t rs, cs;
-  size_t part_bytes, q_off, total;
+  size_t q_off, total;
 };
 
+// The plan of a launch of `mats` matrices (at most kMaxMats; the rest of a
+// longer list goes into further launches).
 OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   OrthoPlan p{};
   const bool tall = rows > cols;
@@ -1270,17 +1272,28 @@ OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   p.NB = ortho::row_blocks(p.R);
   p.mats = (int)std::min<int64_t>(count, ortho::kMaxMats);
   const int kc = ortho::chunk_cols(p.NB);
-  const int chunks = (p.C + kc - 1) / kc;
-  // enough CTAs to fill the device a few times over, at most 32 partial sums
-  // for the iteration kernel's one CTA to add
-  int slices = (int)std::min<int64_t>({(int64_t)chunks, 32, (4 * (int64_t)sms + p.mats - 1) / std::max(1, p.mats)});
-  slices = std::max(1, slices);
-  p.chunks_per_slice = (chunks + slices - 1) / slices;
-  p.slices = (chunks + p.chunks_per_slice - 1) / p.chunks_per_slice;
-  p.part_bytes = (size_t)p.mats * p.slices * ortho::lower_blocks(p.NB) * 64 * sizeof(double);
-  p.q_off = align_up(p.part_bytes, kWsAlign);
-  p.total = align_up(p.q_off + (size_t)p.mats * 64 * p.NB * p.NB * sizeof(float), kWsAlign);
+  p.chunks = (p.C + kc - 1) / kc;
+  // As many CTAs as the device holds, but at most 32 to a matrix: the iteration
+  // kernel's one CTA adds their partial sums.
+  const int64_t all = (int64_t)p.mats * p.chunks;
+  p.gram_ctas = (int)std::min<int64_t>({all, (int64_t)sms * ortho::gram_occupancy(p.NB), (int64_t)32 * p.mats});
+  // A matrix's chunks lie in at most this many shares: a share has at least
+  // all / gram_ctas of them, and one more may begin or end inside the matrix.
+  const int64_t least = all / p.gram_ctas;
+  p.segments = (int)((p.chunks + least - 1) / least + 1);
+  p.apply_ctas = (int)std::min<int64_t>((int64_t)p.mats * ((p.C + ortho::kApplyCols - 1) / ortho::kApplyCols),
+                                        (int64_t)sms * ortho::apply_occupancy(p.NB));
+  p.q_off = align_up((size_t)p.mats * p.segments * ortho::lower_blocks(p.NB) * 64 * sizeof(double), kWsAlign);
+  p.total = align_up(p.q_off + (size_t)p.mats * 64 * p.NB * p.NB * sizeof(double), kWsAlign);
   return p;
+}
+
+// Workspace of a list: its launches follow one another and share it.
+size_t ortho_workspace(int64_t count, int rows, int cols, int sms) {
+  size_t most = ortho_plan(count, rows, cols, sms).total;
+  if (count > ortho::kMaxMats && count % ortho::kMaxMats)
+    most = std::max(most, ortho_plan(count % ortho::kMaxMats, rows, cols, sms).total);
+  return most;
 }
 
 int ortho_check(int64_t count, int32_t rows, int32_t cols) {
@@ -1299,11 +1312,8 @@ int ortho_check_coeffs(const double* coeffs, int32_t steps, double eps) {
 constexpr int kDefaultSmem = 48 * 1024;   // dynamic shared memory a kernel may have without asking
 
 template <int NB, class T, class TO, bool kMom>
-int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, int mats, bool vec,
-                 cudaStream_t s) {
-  const dim3 grid(pl.slices, mats);
-  constexpr int gs = (int)ortho::gram_smem<NB>(), ns = (int)ortho::ns_smem<NB>();
-  constexpr int as = 64 * NB * NB * (int)sizeof(float2), cols = 2 * ortho::apply_threads(NB);
+int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, cudaStream_t s) {
+  constexpr int gs = (int)ortho::gram_smem<NB>(), ns = (int)ortho::ns_smem<NB>(), as = (int)ortho::apply_smem<NB>();
   auto gram = vec ? ortho::gram_kernel<NB, T, kMom, true> : ortho::gram_kernel<NB, T, kMom, false>;
   auto iterate = ortho::iterate_kernel<NB>;
   auto apply = vec ? ortho::apply_kernel<NB, T, TO, kMom, true> : ortho::apply_kernel<NB, T, TO, kMom, false>;
@@ -1311,25 +1321,24 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
   if (ns > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(iterate, cudaFuncAttributeMaxDynamicSharedMemorySize, ns));
   if (as > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
   int st;
-  gram<<<grid, ortho::kThreads, gs, s>>>(p, m);
+  gram<<<pl.gram_ctas, ortho::kThreads, gs, s>>>(p, m);
   if ((st = after_launch())) return st;
-  iterate<<<mats, ortho::kNsThreads, ns, s>>>(p);
+  iterate<<<pl.mats, ortho::kNsThreads, ns, s>>>(p);
   if ((st = after_launch())) return st;
-  apply<<<dim3((pl.C + cols - 1) / cols, mats), ortho::apply_threads(NB), as, s>>>(p, m);
+  apply<<<pl.apply_ctas, ortho::kThreads, as, s>>>(p, m);
   return after_launch();
 }
 
 template <class T, class TO, bool kMom>
-int ortho_dispatch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, int mats, bool vec,
-                   cudaStream_t s) {
+int ortho_dispatch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, cudaStream_t s) {
   switch (pl.NB) {
-    case 1: return ortho_launch<1, T, TO, kMom>(pl, p, m, mats, vec, s);
-    case 2: return ortho_launch<2, T, TO, kMom>(pl, p, m, mats, vec, s);
-    case 3: return ortho_launch<3, T, TO, kMom>(pl, p, m, mats, vec, s);
-    case 5: return ortho_launch<5, T, TO, kMom>(pl, p, m, mats, vec, s);
-    case 6: return ortho_launch<6, T, TO, kMom>(pl, p, m, mats, vec, s);
-    case 8: return ortho_launch<8, T, TO, kMom>(pl, p, m, mats, vec, s);
-    default: return ortho_launch<10, T, TO, kMom>(pl, p, m, mats, vec, s);
+    case 1: return ortho_launch<1, T, TO, kMom>(pl, p, m, vec, s);
+    case 2: return ortho_launch<2, T, TO, kMom>(pl, p, m, vec, s);
+    case 3: return ortho_launch<3, T, TO, kMom>(pl, p, m, vec, s);
+    case 5: return ortho_launch<5, T, TO, kMom>(pl, p, m, vec, s);
+    case 6: return ortho_launch<6, T, TO, kMom>(pl, p, m, vec, s);
+    case 8: return ortho_launch<8, T, TO, kMom>(pl, p, m, vec, s);
+    default: return ortho_launch<10, T, TO, kMom>(pl, p, m, vec, s);
   }
 }
 
@@ -1377,20 +1386,22 @@ int ortho_overlap(const OrthoLists& l, int64_t count, size_t elems, bool same) {
 int dbg_register_list(const void* const* ptrs, const size_t* sizes, int count, cudaStream_t s);
 #endif
 
-int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Params& p, void* workspace, int sms,
-              cudaStream_t s) {
-  const OrthoPlan pl = ortho_plan(count, rows, cols, sms);
+int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Params& p, void* workspace,
+              [[maybe_unused]] size_t workspace_bytes, int sms, cudaStream_t s) {
   char* ws = static_cast<char*>(workspace);
-  p.R = pl.R;
-  p.C = pl.C;
-  p.rs = pl.rs;
-  p.cs = pl.cs;
-  p.slices = pl.slices;
-  p.chunks_per_slice = pl.chunks_per_slice;
-  p.part = reinterpret_cast<double*>(ws);
-  p.q = reinterpret_cast<float*>(ws + pl.q_off);
-  for (int64_t i0 = 0; i0 < count; i0 += pl.mats) {
-    const int mats = (int)std::min<int64_t>(pl.mats, count - i0);
+  for (int64_t i0 = 0; i0 < count; i0 += ortho::kMaxMats) {
+    const OrthoPlan pl = ortho_plan(count - i0, rows, cols, sms);
+    const int mats = pl.mats;
+    p.R = pl.R;
+    p.C = pl.C;
+    p.rs = pl.rs;
+    p.cs = pl.cs;
+    p.mats = mats;
+    p.chunks = pl.chunks;
+    p.gram_ctas = pl.gram_ctas;
+    p.segments = pl.segments;
+    p.part = reinterpret_cast<double*>(ws);
+    p.q = reinterpret_cast<double*>(ws + pl.q_off);
     ortho::Mats m{};
     // pieces of four columns: rows that start on a multiple of four elements
     bool vec = pl.cs == 1 && pl.C % 4 == 0;
@@ -1412,7 +1423,7 @@ int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Par
         ptrs[n] = m.out[i], sizes[n++] = elems * dtype_bytes(l.out_dtype);
         ptrs[n] = m.mom[i], sizes[n++] = elems * 4;
       }
-      ptrs[n] = ws, sizes[n++] = pl.total;
+      ptrs[n] = ws, sizes[n++] = workspace_bytes;
       ptrs[n] = p.lr_dev, sizes[n++] = 4;
       if (int st = dbg_register_list(ptrs, sizes, n, s)) return st;
     }
@@ -1420,14 +1431,14 @@ int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Par
     int st;
     const bool gf = l.grad_dtype == MHC_F32, of = l.out_dtype == MHC_F32;
     if (!l.moms)
-      st = gf ? ortho_dispatch<float, float, false>(pl, p, m, mats, vec, s)
-              : ortho_dispatch<uint16_t, uint16_t, false>(pl, p, m, mats, vec, s);
+      st = gf ? ortho_dispatch<float, float, false>(pl, p, m, vec, s)
+              : ortho_dispatch<uint16_t, uint16_t, false>(pl, p, m, vec, s);
     else if (gf)
-      st = of ? ortho_dispatch<float, float, true>(pl, p, m, mats, vec, s)
-              : ortho_dispatch<float, uint16_t, true>(pl, p, m, mats, vec, s);
+      st = of ? ortho_dispatch<float, float, true>(pl, p, m, vec, s)
+              : ortho_dispatch<float, uint16_t, true>(pl, p, m, vec, s);
     else
-      st = of ? ortho_dispatch<uint16_t, float, true>(pl, p, m, mats, vec, s)
-              : ortho_dispatch<uint16_t, uint16_t, true>(pl, p, m, mats, vec, s);
+      st = of ? ortho_dispatch<uint16_t, float, true>(pl, p, m, vec, s)
+              : ortho_dispatch<uint16_t, uint16_t, true>(pl, p, m, vec, s);
     if (st) return st;
   }
   return MHC_OK;
@@ -1446,7 +1457,7 @@ int ortho_check_lists(const OrthoLists& l, int64_t count, int rows, int cols, bo
   if (int st = ortho_overlap(l, count, (size_t)rows * cols, same)) return st;
   if (!workspace) return MHC_ERR_NULL_POINTER;
   if (!aligned(workspace, kWsAlign)) return MHC_ERR_MISALIGNED;
-  if (workspace_bytes < ortho_plan(count, rows, cols, sms).total) return MHC_ERR_WORKSPACE_TOO_SMALL;
+  if (workspace_bytes < ortho_workspace(count, rows, cols, sms)) return MHC_ERR_WORKSPACE_TOO_SMALL;
   return MHC_OK;
 }
 
@@ -2008,7 +2019,7 @@ int mhc_ortho_workspace_size(int64_t count, int32_t rows, int32_t cols, size_t* 
   if (st) return st;
   int sms = 0;
   if ((st = current_sm_count(&sms))) return st;
-  *bytes = count == 0 || rows == 0 || cols == 0 ? 0 : ortho_plan(count, rows, cols, sms).total;
+  *bytes = count == 0 || rows == 0 || cols == 0 ? 0 : ortho_workspace(count, rows, cols, sms);
   return MHC_OK;
 }
 
@@ -2027,7 +2038,8 @@ int mhc_orthogonalize(const mhc_ortho_args* a, void* stream) {
   p.steps = a->steps;
   p.eps = a->eps;
   std::copy(a->coeffs, a->coeffs + 3 * a->steps, p.coeffs);
-  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, sms, static_cast<cudaStream_t>(stream));
+  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, a->workspace_bytes, sms,
+                   static_cast<cudaStream_t>(stream));
 }
 
 int mhc_muon_step(const mhc_muon_args* a, void* stream) {
@@ -2054,7 +2066,8 @@ int mhc_muon_step(const mhc_muon_args* a, void* stream) {
   p.lr_dev = a->lr_device;
   p.decay = a->weight_decay;
   p.scale = a->scale;
-  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, sms, static_cast<cudaStream_t>(stream));
+  return ortho_run(l, a->count, a->rows, a->cols, p, a->workspace, a->workspace_bytes, sms,
+                   static_cast<cudaStream_t>(stream));
 }
 
 int mhc_debug_bounds(uint64_t* record, int clear) {

@@ -15,9 +15,11 @@
 // The price is precision: A_0 holds the squares of the singular values, and the
 // iteration lifts a small one a few hundred times, so what rounding takes from
 // a small eigenvalue of A_0 is lifted with it (32-bit sums: up to about a
-// percent of a singular value near 1/500 of the norm).  The Gram product and
-// the iteration therefore run in 64 bits, on the double-precision matrix
-// instruction (8 x 8 x 4); only the application, which lifts nothing, is in 32.
+// percent of a singular value near 1/500 of the norm); and in the application
+// the strong directions cancel (32-bit sums: 3e-6 of the result, measured).  So
+// all three run in 64 bits, on the double-precision matrix instruction
+// (8 x 8 x 4), 18.5 T multiply-adds a second here against 34.5 of the scalar
+// 32-bit ones; with few rows memory bounds the two passes over U all the same.
 #pragma once
 
 #include "common.cuh"
@@ -49,10 +51,12 @@ struct Mats {
 struct Params {
   int R, C;                  // short and long side
   int64_t rs, cs;            // element (i, k) of the short x long view is at i * rs + k * cs
-  int slices;                // Gram partial sums per matrix
-  int chunks_per_slice;
-  double* part;              // [L][slices][blocks][64]
-  float* q;                  // [L][P][P], P = 8 * NB
+  int mats;                  // matrices of this launch
+  int chunks;                // column chunks of a matrix in the Gram pass
+  int gram_ctas;             // CTAs that share the mats * chunks chunks
+  int segments;              // Gram partial sums per matrix at most
+  double* part;              // [mats][segments][blocks][64]
+  double* q;                 // [mats][P][P], P = 8 * NB
   float momentum;            // the update's coefficients; unused when only orthogonalising
   int nesterov;
   float lr, decay, scale;
@@ -62,6 +66,11 @@ struct Params {
   double coeffs[3 * kMaxSteps];
 };
 
+// Equal shares of a list of `total` items for `n` takers: taker i has [share(i), share(i + 1)).
+__host__ __device__ __forceinline__ int64_t share(int64_t total, int n, int64_t i) { return total * i / n; }
+// The taker of item x: the largest i with share(i) <= x.
+__device__ __forceinline__ int taker(int64_t total, int n, int64_t x) { return (int)(((x + 1) * n - 1) / total); }
+
 // 8-row blocks, rounded up to the sizes compiled (n = 1 .. 8 need 1 1 2 3 5 6 8 10).
 inline int row_blocks(int R) {
   const int nb = (R + 7) / 8;
@@ -70,6 +79,8 @@ inline int row_blocks(int R) {
 constexpr int lower_blocks(int NB) { return NB * (NB + 1) / 2; }
 // Columns of one staged chunk: about 16 to 24 KB a chunk.
 constexpr int chunk_cols(int NB) { return NB <= 2 ? 256 : NB <= 5 ? 128 : 64; }
+// CTAs on an SM that the kernels' registers are bounded for.
+constexpr int gram_occupancy(int NB) { return NB <= 3 ? 3 : NB <= 6 ? 2 : 1; }
 // Warps that share one set of columns: more than 21 blocks of accumulators (84
 // registers) are split over two warps by block rows.
 constexpr int gram_roles(int NB) { return NB > 6 ? 2 : 1; }
@@ -84,26 +95,66 @@ __device__ __forceinline__ void dmma(double (&d)[2], double a, double b) {
                : "d"(a), "d"(b));
 }
 
+// Four neighbouring elements of a row of the long side as they lie in memory.
+template <class T>
+struct Raw4 {
+  using V = std::conditional_t<std::is_same_v<T, float>, float4, uint2>;
+  V v;
+  __device__ __forceinline__ void unpack(float (&f)[4]) const {
+    if constexpr (std::is_same_v<T, float>) {
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    } else {
+      f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+      f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&f)[4]) {
+    if constexpr (std::is_same_v<T, float>) {
+      v = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+      v.x = pack_bf16x2(f[0], f[1]);
+      v.y = pack_bf16x2(f[2], f[3]);
+    }
+  }
+};
 template <class T>
 __device__ __forceinline__ float ld1(const T* p) {
   if constexpr (std::is_same_v<T, float>) return MHC_LD(p);
   else return bf16_bits_to_f32(MHC_LD(p));
 }
 template <class T>
-__device__ __forceinline__ void ld4(const T* p, float (&f)[4]) {
-  if constexpr (std::is_same_v<T, float>) {
-    const float4 v = MHC_LD(reinterpret_cast<const float4*>(p));
-    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-  } else {
-    const uint2 v = MHC_LD(reinterpret_cast<const uint2*>(p));
-    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
-    f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
-  }
-}
-template <class T>
 __device__ __forceinline__ void st1(T* p, float v) {
   if constexpr (std::is_same_v<T, float>) MHC_ST(p, v);
   else MHC_ST(p, f32_to_bf16_bits(v));
+}
+// Elements (r, c .. c + 3); zeros beyond the matrix.  kVec: rows of cs = 1 that
+// start on a multiple of four elements and have a multiple of four of them.
+template <bool kVec, class T>
+__device__ __forceinline__ void load4(Raw4<T>& raw, const T* base, const Params& P, int r, int64_t c) {
+  raw.v = {};
+  if constexpr (kVec) {
+    if (r < P.R && c < P.C) raw.v = MHC_LD(reinterpret_cast<const typename Raw4<T>::V*>(base + r * P.rs + c));
+  } else {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      f[j] = r < P.R && c + j < P.C ? ld1(base + r * P.rs + (c + j) * P.cs) : 0.f;
+    raw.pack(f);
+  }
+}
+template <bool kVec, class T>
+__device__ __forceinline__ void store4(T* base, const Params& P, int r, int64_t c, const float (&f)[4]) {
+  if constexpr (kVec) {
+    if (r < P.R && c < P.C) {
+      Raw4<T> raw;
+      raw.pack(f);
+      MHC_ST(reinterpret_cast<typename Raw4<T>::V*>(base + r * P.rs + c), raw.v);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r < P.R && c + j < P.C) st1(base + r * P.rs + (c + j) * P.cs, f[j]);
+  }
 }
 
 // momentum and the matrix that is orthogonalised, the same rounding in every
@@ -154,91 +205,102 @@ constexpr size_t gram_smem() {
   return tiles > sums ? tiles : sums;
 }
 
-// Partial Gram products.  Grid (slices, matrices).  A CTA walks its chunks of
-// columns through two shared-memory tiles (the next chunk's loads are in
-// registers while the warps multiply this one), each warp taking its share of a
-// chunk's columns.  With momentum the kernel also forms and writes the new
-// momentum; only this kernel's thread that loads an element writes it.
+// Partial Gram products.  The matrices' chunks of columns are one list of which
+// every CTA takes an equal share; a share that ends inside a matrix leaves a
+// partial sum there.  A CTA walks its chunks through two shared-memory tiles:
+// the next chunk's loads are in flight while the warps multiply this one, each
+// taking its share of a chunk's columns.  With momentum the kernel also forms
+// and writes the new momentum; the thread that loads an element writes it.
 template <int NB, class T, bool kMom, bool kVec>
-__global__ void __launch_bounds__(kThreads) gram_kernel(const __grid_constant__ Params P,
-                                                        const __grid_constant__ Mats M) {
-  constexpr int kRows = 8 * NB, KC = chunk_cols(NB), kStride = KC + 4;
+__global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(const __grid_constant__ Params P,
+                                                                           const __grid_constant__ Mats M) {
+  constexpr int kRows = 8 * NB, KC = chunk_cols(NB), kStride = KC + 4, kB = lower_blocks(NB);
   constexpr int kRoles = gram_roles(NB), kColWarps = kWarps / kRoles, kWarpCols = KC / kColWarps;
   constexpr int kPer = kRows * (KC / 4) / kThreads;   // 4-element pieces of a chunk per thread
   static_assert(kRows * (KC / 4) % kThreads == 0 && kWarpCols % 4 == 0, "chunk split");
   extern __shared__ __align__(16) unsigned char smem[];
   float* tile = reinterpret_cast<float*>(smem);       // two of [kRows][kStride]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int mat = blockIdx.y;
-  const T* g = static_cast<const T*>(M.grad[mat]);
-  float* mom = kMom ? M.mom[mat] : nullptr;
-  const int chunks = (P.C + KC - 1) / KC;
-  const int c0 = blockIdx.x * P.chunks_per_slice, c1 = min(c0 + P.chunks_per_slice, chunks);
+  const int64_t total = (int64_t)P.mats * P.chunks;
+  const int64_t x0 = share(total, P.gram_ctas, blockIdx.x), x1 = share(total, P.gram_ctas, blockIdx.x + 1);
 
-  float reg[kPer][4];
-  auto fetch = [&](int chunk) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = chunk * KC + (e % (KC / 4)) * 4;
-      if (kVec && r < P.R && c < P.C) {   // C is a multiple of 4 here
-        const int64_t o = r * P.rs + c;
-        ld4(g + o, reg[i]);
-        if (kMom) {
-          float m[4];
-          ld4(mom + o, m);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            m[j] = new_momentum(m[j], reg[i][j], P.momentum);
-            reg[i][j] = update_of(m[j], reg[i][j], P.momentum, P.nesterov);
-          }
-          MHC_ST(reinterpret_cast<float4*>(mom + o), make_float4(m[0], m[1], m[2], m[3]));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          reg[i][j] = 0.f;
-          if (!kVec && r < P.R && c + j < P.C) {
-            const int64_t o = r * P.rs + (c + j) * P.cs;
-            const float gv = ld1(g + o);
-            reg[i][j] = gv;
-            if (kMom) {
-              const float m1 = new_momentum(MHC_LD(mom + o), gv, P.momentum);
-              reg[i][j] = update_of(m1, gv, P.momentum, P.nesterov);
-              MHC_ST(mom + o, m1);
-            }
-          }
-        }
-      }
-    }
-  };
-  auto stage = [&](float* dst) {
+  Raw4<T> g[kPer];
+  Raw4<float> m[kPer];
+  auto fetch = [&](int64_t x) {
+    const int mat = (int)(x / P.chunks);
+    const int64_t col = (x - (int64_t)mat * P.chunks) * KC;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * 4;
-      *reinterpret_cast<float4*>(dst + r * kStride + c) = make_float4(reg[i][0], reg[i][1], reg[i][2], reg[i][3]);
+      load4<kVec>(g[i], static_cast<const T*>(M.grad[mat]), P, r, col + c);
+      if (kMom) load4<kVec>(m[i], static_cast<const float*>(M.mom[mat]), P, r, col + c);
+    }
+  };
+  auto stage = [&](int64_t x, float* dst) {
+    const int mat = (int)(x / P.chunks);
+    const int64_t col = (x - (int64_t)mat * P.chunks) * KC;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * 4;
+      float f[4];
+      g[i].unpack(f);
+      if (kMom) {
+        float m1[4];
+        m[i].unpack(m1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m1[j] = new_momentum(m1[j], f[j], P.momentum);
+          f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
+        }
+        store4<kVec>(M.mom[mat], P, r, col + c, m1);
+      }
+      *reinterpret_cast<float4*>(dst + r * kStride + c) = make_float4(f[0], f[1], f[2], f[3]);
     }
   };
 
-  double* sums = reinterpret_cast<double*>(smem) + (size_t)(warp / kRoles) * lower_blocks(NB) * 64;
+  const int cw = warp / kRoles;
+  double* sums = reinterpret_cast<double*>(smem) + (size_t)cw * kB * 64;
+  // The matrix's sum over this CTA's chunks: the column warps' in warp order.
+  auto finish = [&](int mat, auto& gram) {
+    __syncthreads();   // the tiles have been read
+    gram.store(sums, lane);
+    __syncthreads();
+    const int first = taker(total, P.gram_ctas, (int64_t)mat * P.chunks);
+    double* dst = P.part + ((int64_t)mat * P.segments + (blockIdx.x - first)) * (kB * 64);
+    for (int i = threadIdx.x; i < kB * 64; i += kThreads) {
+      double v = 0.0;
+#pragma unroll
+      for (int w = 0; w < kColWarps; ++w) v += reinterpret_cast<const double*>(smem)[w * kB * 64 + i];
+      MHC_ST(dst + i, v);
+    }
+    __syncthreads();
+    gram.clear();
+  };
   // One role's whole walk, so that a warp holds its own accumulators only; both
   // roles pass the same number of barriers.
   auto walk = [&](auto gram) {
     gram.clear();
-    const int col0 = (warp / kRoles) * kWarpCols;
-    if (c0 < c1) {
-      fetch(c0);
-      stage(tile);
-      __syncthreads();
-      for (int c = c0; c < c1; ++c) {
-        float* cur = tile + ((c - c0) & 1) * kRows * kStride;
-        float* nxt = tile + ((c - c0 + 1) & 1) * kRows * kStride;
-        if (c + 1 < c1) fetch(c + 1);
-        gram.run(cur + col0, kStride, kWarpCols, lane);
-        if (c + 1 < c1) stage(nxt);   // last read in the round before, ended by its barrier
+    if (x0 < x1) fetch(x0);
+    bool staged = false;
+    for (int64_t x = x0; x < x1; ++x) {
+      float* cur = tile + ((x - x0) & 1) * kRows * kStride;
+      float* nxt = tile + ((x - x0 + 1) & 1) * kRows * kStride;
+      if (!staged) {
+        stage(x, cur);
+        __syncthreads();
+      }
+      const int mat = (int)(x / P.chunks);
+      const bool last = x + 1 == x1 || (int)((x + 1) / P.chunks) != mat;
+      if (x + 1 < x1) fetch(x + 1);
+      gram.run(cur + cw * kWarpCols, kStride, kWarpCols, lane);
+      staged = !last;
+      if (last) {
+        finish(mat, gram);   // the sums lie over the tiles: the next chunk is staged after them
+      } else {
+        stage(x + 1, nxt);   // last read in the round before, ended by its barrier
         __syncthreads();
       }
     }
-    gram.store(sums, lane);
   };
   if constexpr (kRoles == 1) {
     walk(Gram<0, NB>{});
@@ -247,15 +309,6 @@ __global__ void __launch_bounds__(kThreads) gram_kernel(const __grid_constant__ 
       walk(Gram<0, role_split(NB)>{});
     else
       walk(Gram<role_split(NB), NB>{});
-  }
-  // sum over the column warps in warp order
-  __syncthreads();
-  double* dst = P.part + ((int64_t)mat * P.slices + blockIdx.x) * (lower_blocks(NB) * 64);
-  for (int i = threadIdx.x; i < lower_blocks(NB) * 64; i += kThreads) {
-    double v = 0.0;
-#pragma unroll
-    for (int w = 0; w < kColWarps; ++w) v += reinterpret_cast<const double*>(smem)[w * lower_blocks(NB) * 64 + i];
-    MHC_ST(dst + i, v);
   }
 }
 
@@ -322,14 +375,17 @@ __global__ void __launch_bounds__(kNsThreads) iterate_kernel(const __grid_consta
   double* Q = W + kRows * S;
   __shared__ double inv_norm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const double* part = P.part + (int64_t)blockIdx.x * P.slices * (kB * 64);
+  const double* part = P.part + (int64_t)blockIdx.x * P.segments * (kB * 64);
+  const int64_t total = (int64_t)P.mats * P.chunks, c0 = (int64_t)blockIdx.x * P.chunks;
+  const int segments = taker(total, P.gram_ctas, c0 + P.chunks - 1) - taker(total, P.gram_ctas, c0) + 1;
   auto both = [&](double* X, int r, int c, double v) {
     X[r * S + c] = v;
     X[c * S + r] = v;
   };
   for (int e = threadIdx.x; e < kB * 64; e += kNsThreads) {
     double v = 0.0;
-    for (int s = 0; s < P.slices; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64) + e);
+#pragma unroll 8
+    for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64) + e);
     int i, j;
     Product<NB>::block(e / 64, i, j);
     const int l = (e & 63) >> 1;
@@ -370,110 +426,111 @@ __global__ void __launch_bounds__(kNsThreads) iterate_kernel(const __grid_consta
       __syncthreads();
     }
   }
-  float* q = P.q + (int64_t)blockIdx.x * kRows * kRows;
-  for (int e = threadIdx.x; e < kRows * kRows; e += kNsThreads) {
-    const int r = e / kRows, c = e % kRows;
-    const bool in = r < P.R && c < P.R;   // beyond the matrix: the a_k on the padded diagonal
-    MHC_ST(q + e, in ? (float)(Q[r * S + c] * inv) : 0.f);
-  }
+  double* q = P.q + (int64_t)blockIdx.x * kRows * kRows;
+  for (int e = threadIdx.x; e < kRows * kRows; e += kNsThreads) MHC_ST(q + e, Q[e / kRows * S + e % kRows] * inv);
 }
 
-// O = Q U on two columns per thread (kVec: neighbours, else kThreads apart),
-// and what is made of it: the output, or the parameter's update
+// O = Q U and what is made of it: the output, or the parameter's update
 //   p' = (1 - lr decay) p - lr scale O.
-constexpr int apply_threads(int NB) { return NB > 6 ? 128 : 256; }
+// A warp takes 32 columns at a time.  Lane l loads four neighbouring columns
+// 4 (l / 4) .. of row 4 k + l % 4, which are its B fragments of four 8-column
+// products whose columns lie four apart; their results leave it eight
+// neighbouring columns 8 (l % 4) .. of rows l / 4 + 8 i.  So both ends are whole
+// vectors and nothing goes through shared memory but Q.
+constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
+constexpr int apply_ahead(int NB) { return NB <= 3 ? 2 * NB : 4; }   // row loads in flight
+template <int NB>
+constexpr size_t apply_smem() {
+  return (size_t)(8 * NB) * ns_stride(NB) * sizeof(double);
+}
+constexpr int kApplyCols = 32 * kWarps;   // columns of a CTA's step
 template <int NB, class T, class TO, bool kMom, bool kVec>
-__global__ void __launch_bounds__(apply_threads(NB)) apply_kernel(const __grid_constant__ Params P,
-                                                                  const __grid_constant__ Mats M) {
-  constexpr int kRows = 8 * NB, kT = apply_threads(NB);
+__global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(const __grid_constant__ Params P,
+                                                                             const __grid_constant__ Mats M) {
+  constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB);
   extern __shared__ __align__(16) unsigned char smem[];
-  float2* q = reinterpret_cast<float2*>(smem);   // [kRows][kRows], each value twice (packed products)
-  const int mat = blockIdx.y;
-  const T* g = static_cast<const T*>(M.grad[mat]);
-  const float* mom = kMom ? M.mom[mat] : nullptr;
-  TO* out = static_cast<TO*>(M.out[mat]);
-  const float* qs = P.q + (int64_t)mat * kRows * kRows;
-  const int64_t base = (int64_t)blockIdx.x * (2 * kT);
-  const int64_t ca = kVec ? base + 2 * threadIdx.x : base + threadIdx.x, cb = kVec ? ca + 1 : ca + kT;
-  float2 u[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    u[r] = make_float2(0.f, 0.f);
-    if (r < P.R) {
-      float gv[2] = {0.f, 0.f}, m[2] = {0.f, 0.f};
-      if constexpr (kVec) {
-        if (ca < P.C) {
-          const int64_t o = r * P.rs + ca;
-          if constexpr (std::is_same_v<T, float>) {
-            const float2 v = MHC_LDG(reinterpret_cast<const float2*>(g + o));
-            gv[0] = v.x, gv[1] = v.y;
-          } else {
-            const uint32_t v = MHC_LDG(reinterpret_cast<const uint32_t*>(g + o));
-            gv[0] = __uint_as_float(v << 16), gv[1] = __uint_as_float(v & 0xFFFF0000u);
-          }
-          if (kMom) {
-            const float2 v = MHC_LDG(reinterpret_cast<const float2*>(mom + o));
-            m[0] = v.x, m[1] = v.y;
-          }
-        }
-      } else {
-        const int64_t oa = r * P.rs + ca * P.cs, ob = r * P.rs + cb * P.cs;
-        if (ca < P.C) gv[0] = ld1(g + oa);
-        if (cb < P.C) gv[1] = ld1(g + ob);
-        if (kMom) {
-          if (ca < P.C) m[0] = MHC_LD(mom + oa);
-          if (cb < P.C) m[1] = MHC_LD(mom + ob);
-        }
-      }
-      u[r] = kMom ? make_float2(update_of(m[0], gv[0], P.momentum, P.nesterov),
-                                update_of(m[1], gv[1], P.momentum, P.nesterov))
-                  : make_float2(gv[0], gv[1]);
-    }
-  }
-  for (int e = threadIdx.x; e < kRows * kRows; e += kT) {
-    const float v = MHC_LDG(qs + e);
-    q[e] = make_float2(v, v);
-  }
-  __syncthreads();
+  double* Q = reinterpret_cast<double*>(smem);   // [kRows][S]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int steps = (P.C + kApplyCols - 1) / kApplyCols;
+  const int64_t total = (int64_t)P.mats * steps;
+  const int64_t x0 = share(total, gridDim.x, blockIdx.x), x1 = share(total, gridDim.x, blockIdx.x + 1);
   float keep = 0.f, step = 0.f;
   if (kMom) {
     const float lr = P.lr_dev ? MHC_LDG(P.lr_dev) : P.lr;
     keep = 1.f - lr * P.decay;
     step = -lr * P.scale;
   }
-  for (int r = 0; r < P.R; ++r) {
-    const float4* qr = reinterpret_cast<const float4*>(q + r * kRows);
-    float2 o0 = make_float2(0.f, 0.f), o1 = o0;
+  int loaded = -1;
+  for (int64_t x = x1 - 1; x >= x0; --x) {
+    const int mat = (int)(x / steps);
+    const int64_t col = (x - (int64_t)mat * steps) * kApplyCols + warp * 32;
+    const T* grad = static_cast<const T*>(M.grad[mat]);
+    TO* out = static_cast<TO*>(M.out[mat]);
+    Raw4<T> g[kAhead];
+    Raw4<float> m[kAhead];
+    auto fetch = [&](int k) {
+      load4<kVec>(g[k % kAhead], grad, P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
+      if (kMom) load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
+    };
 #pragma unroll
-    for (int k = 0; k < kRows; k += 2) {
-      const float4 w = qr[k / 2];
-      o0 = __ffma2_rn(make_float2(w.x, w.y), u[k], o0);
-      o1 = __ffma2_rn(make_float2(w.z, w.w), u[k + 1], o1);
+    for (int k = 0; k < kAhead; ++k) fetch(k);
+    if (mat != loaded) {   // the same for the whole CTA
+      __syncthreads();
+      const double* q = P.q + (int64_t)mat * kRows * kRows;
+      for (int e = threadIdx.x; e < kRows * kRows; e += kThreads) Q[e / kRows * S + e % kRows] = MHC_LD(q + e);
+      __syncthreads();
+      loaded = mat;
     }
-    float v0 = o0.x + o1.x, v1 = o0.y + o1.y;
-    if constexpr (kVec) {
-      if (ca < P.C) {
-        const int64_t o = r * P.rs + ca;
-        if constexpr (std::is_same_v<TO, float>) {
-          if (kMom) {
-            const float2 p = MHC_LD(reinterpret_cast<const float2*>(out + o));
-            v0 = fmaf(keep, p.x, step * v0);
-            v1 = fmaf(keep, p.y, step * v1);
-          }
-          MHC_ST(reinterpret_cast<float2*>(out + o), make_float2(v0, v1));
-        } else {
-          if (kMom) {
-            const uint32_t p = MHC_LD(reinterpret_cast<const uint32_t*>(out + o));
-            v0 = fmaf(keep, __uint_as_float(p << 16), step * v0);
-            v1 = fmaf(keep, __uint_as_float(p & 0xFFFF0000u), step * v1);
-          }
-          MHC_ST(reinterpret_cast<uint32_t*>(out + o), pack_bf16x2(v0, v1));
-        }
+    double acc[NB][4][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e][0] = acc[i][e][1] = 0.0;
+    const double* a = Q + (lane >> 2) * S + (lane & 3);
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      float f[4];
+      g[k % kAhead].unpack(f);
+      if (kMom) {
+        float m1[4];
+        m[k % kAhead].unpack(m1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
       }
-    } else {
-      const int64_t oa = r * P.rs + ca * P.cs, ob = r * P.rs + cb * P.cs;
-      if (ca < P.C) st1(out + oa, kMom ? fmaf(keep, ld1(out + oa), step * v0) : v0);
-      if (cb < P.C) st1(out + ob, kMom ? fmaf(keep, ld1(out + ob), step * v1) : v1);
+      if (k + kAhead < kK) fetch(k + kAhead);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const double q = a[8 * i * S + 4 * k];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dmma(acc[i][e], q, (double)f[e]);
+      }
+    }
+    const int64_t oc = col + 8 * (lane & 3);
+    constexpr int kBatch = NB <= 3 ? NB : 2;   // row blocks whose parameters are loaded together
+#pragma unroll
+    for (int i0 = 0; i0 < NB; i0 += kBatch) {
+      Raw4<TO> p[kBatch][2];
+      if (kMom)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (i0 + i < NB)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              load4<kVec>(p[i][j], static_cast<const TO*>(out), P, 8 * (i0 + i) + (lane >> 2), oc + 4 * j);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (i0 + i < NB)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float o[4], old[4];
+            if (kMom) p[i][j].unpack(old);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = (float)acc[i0 + i][e][j];
+              o[e] = kMom ? fmaf(keep, old[e], step * v) : v;
+            }
+            store4<kVec>(out, P, 8 * (i0 + i) + (lane >> 2), oc + 4 * j, o);
+          }
     }
   }
 }
