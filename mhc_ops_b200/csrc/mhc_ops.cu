@@ -1255,9 +1255,9 @@ int rope_dispatch(const mhc_qk_args* a, const rope::Params& p, const RopePlan& r
 
 // ------------------------------------------------------- updates of phi
 struct OrthoPlan {
-  int R, C, NB, chunks, gram_ctas, segments, apply_ctas, mats;   // mats: matrices of one launch
+  int R, C, NB, chunks, gram_ctas, segments, apply_ctas, apply_warps, mats;   // mats: matrices of one launch
   int64_t rs, cs;
-  size_t q_off, total;
+  size_t q_off, exchange_off, total;
 };
 
 // The plan of a launch of `mats` matrices (at most kMaxMats; the rest of a
@@ -1273,18 +1273,24 @@ OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   p.mats = (int)std::min<int64_t>(count, ortho::kMaxMats);
   const int kc = ortho::chunk_cols(p.NB);
   p.chunks = (p.C + kc - 1) / kc;
-  // As many CTAs as the device holds, but at most 32 to a matrix: the iteration
-  // kernel's one CTA adds their partial sums.
+  // As many CTAs as the device holds, but a limit to a matrix's partial sums,
+  // which one CTA adds before the iteration (96 where a cluster shares that).
   const int64_t all = (int64_t)p.mats * p.chunks;
-  p.gram_ctas = (int)std::min<int64_t>({all, (int64_t)sms * ortho::gram_occupancy(p.NB), (int64_t)32 * p.mats});
+  p.gram_ctas = (int)std::min<int64_t>({all, (int64_t)sms * ortho::gram_occupancy(p.NB),
+                                        (int64_t)(p.NB <= ortho::kSmallBlocks ? 32 : 96) * p.mats});
   // A matrix's chunks lie in at most this many shares: a share has at least
   // all / gram_ctas of them, and one more may begin or end inside the matrix.
   const int64_t least = all / p.gram_ctas;
   p.segments = (int)((p.chunks + least - 1) / least + 1);
-  p.apply_ctas = (int)std::min<int64_t>((int64_t)p.mats * ((p.C + ortho::kApplyCols - 1) / ortho::kApplyCols),
-                                        (int64_t)sms * ortho::apply_occupancy(p.NB));
+  // Application: 32 columns to a warp at a time.  Four warps to a CTA, one on each
+  // of an SM's matrix pipes, where that spreads the columns over more SMs.
+  const int64_t width = (p.C + 31) / 32, slots = (int64_t)sms * ortho::apply_occupancy(p.NB);
+  p.apply_warps = (int64_t)p.mats * ((width + 7) / 8) < slots ? 4 : 8;
+  p.apply_ctas = (int)std::min<int64_t>((int64_t)p.mats * ((width + p.apply_warps - 1) / p.apply_warps), slots);
   p.q_off = align_up((size_t)p.mats * p.segments * ortho::lower_blocks(p.NB) * 64 * sizeof(double), kWsAlign);
-  p.total = align_up(p.q_off + (size_t)p.mats * 64 * p.NB * p.NB * sizeof(double), kWsAlign);
+  const size_t square = (size_t)p.mats * 64 * p.NB * p.NB * sizeof(double);
+  p.exchange_off = align_up(p.q_off + square, kWsAlign);
+  p.total = p.exchange_off + (p.NB > ortho::kSmallBlocks ? 2 * square : 0);
   return p;
 }
 
@@ -1311,34 +1317,81 @@ int ortho_check_coeffs(const double* coeffs, int32_t steps, double eps) {
 
 constexpr int kDefaultSmem = 48 * 1024;   // dynamic shared memory a kernel may have without asking
 
+// A launch that may start while its predecessor in the stream still runs (the
+// kernel waits for what it needs), as clusters of `cluster` CTAs when that is above 1.
+template <class... A>
+int launch_behind(void (*kernel)(A...), int ctas, int threads, int smem, int cluster, cudaStream_t s,
+                  const std::decay_t<A>&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  MHC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return after_launch();
+}
+
+template <int NB, int kSP>
+int ortho_iterate_cluster(const OrthoPlan& pl, const ortho::Params& p, cudaStream_t s) {
+  auto kernel = ortho::iterate_cluster_kernel<NB, kSP>;
+  constexpr int smem = (int)ortho::cluster_smem<NB, kSP>(), cluster = NB / kSP;
+  MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (cluster > 8) MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  return launch_behind(kernel, pl.mats * cluster, 64 * NB, smem, cluster, s, p);
+}
+
+template <int NB>
+int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, cudaStream_t s) {
+  if constexpr (NB <= ortho::kSmallBlocks) {
+    auto kernel = ortho::iterate_small_kernel<NB>;
+    constexpr int smem = (int)ortho::small_smem<NB>();
+    if (smem > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return launch_behind(kernel, pl.mats, 32 * ortho::small_warps(NB), smem, 1, s, p);
+  } else {
+    // a row block to a CTA while the device holds all the clusters at once, else two
+    if constexpr (NB % 2 == 0)
+      if (pl.mats * NB > sms) return ortho_iterate_cluster<NB, 2>(pl, p, s);
+    return ortho_iterate_cluster<NB, 1>(pl, p, s);
+  }
+}
+
 template <int NB, class T, class TO, bool kMom>
-int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, cudaStream_t s) {
-  constexpr int gs = (int)ortho::gram_smem<NB>(), ns = (int)ortho::ns_smem<NB>(), as = (int)ortho::apply_smem<NB>();
+int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, int sms,
+                 cudaStream_t s) {
+  constexpr int gs = (int)ortho::gram_smem<NB>();
+  const int as = (int)(vec && kMom ? ortho::apply_smem<NB, TO, true>(pl.apply_warps)
+                                   : ortho::apply_smem<NB, TO, false>(pl.apply_warps));
   auto gram = vec ? ortho::gram_kernel<NB, T, kMom, true> : ortho::gram_kernel<NB, T, kMom, false>;
-  auto iterate = ortho::iterate_kernel<NB>;
   auto apply = vec ? ortho::apply_kernel<NB, T, TO, kMom, true> : ortho::apply_kernel<NB, T, TO, kMom, false>;
   if (gs > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
-  if (ns > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(iterate, cudaFuncAttributeMaxDynamicSharedMemorySize, ns));
   if (as > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
   int st;
   gram<<<pl.gram_ctas, ortho::kThreads, gs, s>>>(p, m);
   if ((st = after_launch())) return st;
-  iterate<<<pl.mats, ortho::kNsThreads, ns, s>>>(p);
-  if ((st = after_launch())) return st;
-  apply<<<pl.apply_ctas, ortho::kThreads, as, s>>>(p, m);
-  return after_launch();
+  if ((st = ortho_iterate<NB>(pl, p, sms, s))) return st;
+  return launch_behind(apply, pl.apply_ctas, 32 * pl.apply_warps, as, 1, s, p, m);
 }
 
 template <class T, class TO, bool kMom>
-int ortho_dispatch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, cudaStream_t s) {
+int ortho_dispatch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, int sms,
+                   cudaStream_t s) {
   switch (pl.NB) {
-    case 1: return ortho_launch<1, T, TO, kMom>(pl, p, m, vec, s);
-    case 2: return ortho_launch<2, T, TO, kMom>(pl, p, m, vec, s);
-    case 3: return ortho_launch<3, T, TO, kMom>(pl, p, m, vec, s);
-    case 5: return ortho_launch<5, T, TO, kMom>(pl, p, m, vec, s);
-    case 6: return ortho_launch<6, T, TO, kMom>(pl, p, m, vec, s);
-    case 8: return ortho_launch<8, T, TO, kMom>(pl, p, m, vec, s);
-    default: return ortho_launch<10, T, TO, kMom>(pl, p, m, vec, s);
+    case 1: return ortho_launch<1, T, TO, kMom>(pl, p, m, vec, sms, s);
+    case 2: return ortho_launch<2, T, TO, kMom>(pl, p, m, vec, sms, s);
+    case 3: return ortho_launch<3, T, TO, kMom>(pl, p, m, vec, sms, s);
+    case 5: return ortho_launch<5, T, TO, kMom>(pl, p, m, vec, sms, s);
+    case 6: return ortho_launch<6, T, TO, kMom>(pl, p, m, vec, sms, s);
+    case 8: return ortho_launch<8, T, TO, kMom>(pl, p, m, vec, sms, s);
+    default: return ortho_launch<10, T, TO, kMom>(pl, p, m, vec, sms, s);
   }
 }
 
@@ -1402,6 +1455,7 @@ int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Par
     p.segments = pl.segments;
     p.part = reinterpret_cast<double*>(ws);
     p.q = reinterpret_cast<double*>(ws + pl.q_off);
+    p.exchange = reinterpret_cast<double*>(ws + pl.exchange_off);
     ortho::Mats m{};
     // pieces of four columns: rows that start on a multiple of four elements
     bool vec = pl.cs == 1 && pl.C % 4 == 0;
@@ -1431,14 +1485,14 @@ int ortho_run(const OrthoLists& l, int64_t count, int rows, int cols, ortho::Par
     int st;
     const bool gf = l.grad_dtype == MHC_F32, of = l.out_dtype == MHC_F32;
     if (!l.moms)
-      st = gf ? ortho_dispatch<float, float, false>(pl, p, m, vec, s)
-              : ortho_dispatch<uint16_t, uint16_t, false>(pl, p, m, vec, s);
+      st = gf ? ortho_dispatch<float, float, false>(pl, p, m, vec, sms, s)
+              : ortho_dispatch<uint16_t, uint16_t, false>(pl, p, m, vec, sms, s);
     else if (gf)
-      st = of ? ortho_dispatch<float, float, true>(pl, p, m, vec, s)
-              : ortho_dispatch<float, uint16_t, true>(pl, p, m, vec, s);
+      st = of ? ortho_dispatch<float, float, true>(pl, p, m, vec, sms, s)
+              : ortho_dispatch<float, uint16_t, true>(pl, p, m, vec, sms, s);
     else
-      st = of ? ortho_dispatch<uint16_t, float, true>(pl, p, m, vec, s)
-              : ortho_dispatch<uint16_t, uint16_t, true>(pl, p, m, vec, s);
+      st = of ? ortho_dispatch<uint16_t, float, true>(pl, p, m, vec, sms, s)
+              : ortho_dispatch<uint16_t, uint16_t, true>(pl, p, m, vec, sms, s);
     if (st) return st;
   }
   return MHC_OK;

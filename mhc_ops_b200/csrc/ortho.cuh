@@ -22,6 +22,8 @@
 // 32-bit ones; with few rows memory bounds the two passes over U all the same.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 #undef MHC_FILE_ID
@@ -39,8 +41,6 @@ constexpr int kMaxMats = 64;     // matrices of one launch (their pointers trave
 #endif
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kNsThreads = 512;
-constexpr int kNsWarps = kNsThreads / 32;
 
 struct Mats {
   const void* grad[kMaxMats];
@@ -57,6 +57,7 @@ struct Params {
   int segments;              // Gram partial sums per matrix at most
   double* part;              // [mats][segments][blocks][64]
   double* q;                 // [mats][P][P], P = 8 * NB
+  double* exchange;          // [mats][2][P][P], what the clusters' CTAs pass on
   float momentum;            // the update's coefficients; unused when only orthogonalising
   int nesterov;
   float lr, decay, scale;
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
       }
     }
   };
+  cudaTriggerProgrammaticLaunchCompletion();   // the iteration waits for this kernel's end itself
   if constexpr (kRoles == 1) {
     walk(Gram<0, NB>{});
   } else {
@@ -315,119 +317,273 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
 // Row stride of an R x R matrix of doubles in shared memory: 4 or 12 modulo 16,
 // so that the four rows a half warp's fragment load touches fall into different banks.
 constexpr int ns_stride(int NB) { return 8 * NB + 4; }
+
+// One 8 x 8 block of X Y^T over all columns: x, y point at the lane's fragment
+// places in X's and Y's row blocks.  Two chains of products, added at the end.
 template <int NB>
-constexpr size_t ns_smem() {
-  return 4 * (size_t)(8 * NB) * ns_stride(NB) * sizeof(double);
+__device__ __forceinline__ void block_product(const double* x, const double* y, double (&d)[2]) {
+  double e[2] = {0.0, 0.0};
+  d[0] = d[1] = 0.0;
+#pragma unroll
+  for (int k = 0; k < 8 * NB; k += 8) {
+    dmma(d, x[k], y[k]);
+    dmma(e, x[k + 4], y[k + 4]);
+  }
+  d[0] += e[0];
+  d[1] += e[1];
+}
+// Partial Gram sums of a matrix.
+__device__ __forceinline__ const double* partials(const Params& P, int mat, int blocks, int& segments) {
+  const int64_t total = (int64_t)P.mats * P.chunks, c0 = (int64_t)mat * P.chunks;
+  segments = taker(total, P.gram_ctas, c0 + P.chunks - 1) - taker(total, P.gram_ctas, c0) + 1;
+  return P.part + (int64_t)mat * P.segments * (blocks * 64);
+}
+// 1 / (|U|_F + eps) from the diagonal, by one warp.
+__device__ __forceinline__ double inverse_norm(const double* A, int rows, int stride, double eps) {
+  double tr = 0.0;
+  for (int i = threadIdx.x & 31; i < rows; i += 32) tr += A[i * stride + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
+  return 1.0 / (sqrt(tr) + eps);
 }
 
-// Lower-triangle blocks of X Y for commuting symmetric X, Y (their product is
-// symmetric and Y's rows serve as its columns); a warp's blocks in registers.
+// The iteration on matrices of up to 40 rows, a CTA each: a warp per block of
+// the lower triangle (products of commuting symmetric matrices are symmetric;
+// Y's rows serve as its columns) and another for the second product of a step.
+// What is left is latency: 13 dependent products of at most 10 instructions.
+constexpr int kSmallBlocks = 5;
+constexpr int small_warps(int NB) { return 2 * lower_blocks(NB); }
 template <int NB>
-struct Product {
-  static constexpr int kPerWarp = (lower_blocks(NB) + kNsWarps - 1) / kNsWarps;
-  double acc[kPerWarp][2];
-  __device__ __forceinline__ static void block(int x, int& i, int& j) {
-    i = 0;
-    while (lower_blocks(i + 1) <= x) ++i;
-    j = x - lower_blocks(i);
-  }
-  __device__ __forceinline__ void run(const double* X, const double* Y, int warp, int lane) {
-    constexpr int S = ns_stride(NB);
-#pragma unroll
-    for (int t = 0; t < kPerWarp; ++t) {
-      const int x = warp + t * kNsWarps;
-      acc[t][0] = acc[t][1] = 0.0;
-      if (x < lower_blocks(NB)) {
-        int i, j;
-        block(x, i, j);
-        const double* a = X + (8 * i + (lane >> 2)) * S + (lane & 3);
-        const double* b = Y + (8 * j + (lane >> 2)) * S + (lane & 3);
-#pragma unroll
-        for (int k = 0; k < 8 * NB; k += 4) dmma(acc[t], a[k], b[k]);
-      }
-    }
-  }
-  // f(row, col, value) for each element of the lower blocks, and its mirror
-  template <class F>
-  __device__ __forceinline__ void each(int warp, int lane, F f) const {
-#pragma unroll
-    for (int t = 0; t < kPerWarp; ++t) {
-      const int x = warp + t * kNsWarps;
-      if (x < lower_blocks(NB)) {
-        int i, j;
-        block(x, i, j);
-        const int r = 8 * i + (lane >> 2), c = 8 * j + 2 * (lane & 3);
-        f(r, c, acc[t][0]);
-        f(r, c + 1, acc[t][1]);
-      }
-    }
-  }
-};
-
-// The iteration on the small matrices, one CTA per matrix.
+constexpr size_t small_smem() {
+  return (size_t)4 * (8 * NB) * ns_stride(NB) * sizeof(double);
+}
 template <int NB>
-__global__ void __launch_bounds__(kNsThreads) iterate_kernel(const __grid_constant__ Params P) {
-  constexpr int kRows = 8 * NB, S = ns_stride(NB), kB = lower_blocks(NB);
+__global__ void __launch_bounds__(32 * small_warps(NB)) iterate_small_kernel(const __grid_constant__ Params P) {
+  constexpr int kRows = 8 * NB, S = ns_stride(NB), kB = lower_blocks(NB), kT = 32 * small_warps(NB);
   extern __shared__ __align__(16) unsigned char smem[];
   double* A = reinterpret_cast<double*>(smem);
-  double* Mk = A + kRows * S;
-  double* W = Mk + kRows * S;
-  double* Q = W + kRows * S;
+  double *Mk = A + kRows * S, *W = Mk + kRows * S, *Q = W + kRows * S;
   __shared__ double inv_norm;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const double* part = P.part + (int64_t)blockIdx.x * P.segments * (kB * 64);
-  const int64_t total = (int64_t)P.mats * P.chunks, c0 = (int64_t)blockIdx.x * P.chunks;
-  const int segments = taker(total, P.gram_ctas, c0 + P.chunks - 1) - taker(total, P.gram_ctas, c0) + 1;
-  auto both = [&](double* X, int r, int c, double v) {
-    X[r * S + c] = v;
-    X[c * S + r] = v;
+  const bool second = warp >= kB;
+  const int x = second ? warp - kB : warp;
+  int bi = 0;
+  while (lower_blocks(bi + 1) <= x) ++bi;
+  const int bj = x - lower_blocks(bi);
+  const int r = 8 * bi + (lane >> 2), c = 8 * bj + 2 * (lane & 3);           // this lane's two results
+  const int fx = (8 * bi + (lane >> 2)) * S + (lane & 3), fy = (8 * bj + (lane >> 2)) * S + (lane & 3);
+  auto put = [&](double* X, double v0, double v1) {   // a result and its mirror image
+    X[r * S + c] = v0;
+    X[r * S + c + 1] = v1;
+    X[c * S + r] = v0;
+    X[(c + 1) * S + r] = v1;
   };
-  for (int e = threadIdx.x; e < kB * 64; e += kNsThreads) {
-    double v = 0.0;
-#pragma unroll 8
-    for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64) + e);
-    int i, j;
-    Product<NB>::block(e / 64, i, j);
-    const int l = (e & 63) >> 1;
-    both(A, 8 * i + (l >> 2), 8 * j + 2 * (l & 3) + (e & 1), v);
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  int segments;
+  const double* part = partials(P, blockIdx.x, kB, segments) + x * 64 + 2 * lane + (second ? 1 : 0);
+  {
+    double v = 0.0;   // first warps: the even elements of their block, second ones the odd
+#pragma unroll 16
+    for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64));
+    const int cc = c + (second ? 1 : 0);
+    A[r * S + cc] = v;
+    A[cc * S + r] = v;
   }
   __syncthreads();
   if (warp == 0) {
-    double tr = 0.0;
-    for (int i = lane; i < kRows; i += 32) tr += A[i * S + i];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) tr += __shfl_xor_sync(0xffffffffu, tr, o);
-    if (lane == 0) inv_norm = 1.0 / (sqrt(tr) + P.eps);
+    const double v = inverse_norm(A, kRows, S, P.eps);
+    if (lane == 0) inv_norm = v;
   }
   __syncthreads();
   const double inv = inv_norm;
-  for (int e = threadIdx.x; e < kRows * kRows; e += kNsThreads) A[(e / kRows) * S + e % kRows] *= inv * inv;
+  for (int e = threadIdx.x; e < kRows * kRows; e += kT) A[e / kRows * S + e % kRows] *= inv * inv;
   __syncthreads();
-  Product<NB> p, p2;
+  double d[2];
   for (int k = 0; k < P.steps; ++k) {
-    const double a = P.coeffs[3 * k], b = P.coeffs[3 * k + 1], c = P.coeffs[3 * k + 2];
-    p.run(A, A, warp, lane);
-    p.each(warp, lane, [&](int r, int col, double v) {
-      v = (r == col ? a : 0.0) + b * A[r * S + col] + c * v;
-      both(Mk, r, col, v);
-      if (k == 0) both(Q, r, col, v);
-    });
-    __syncthreads();
+    const double a = P.coeffs[3 * k], b = P.coeffs[3 * k + 1], cc = P.coeffs[3 * k + 2];
     const bool more = k + 1 < P.steps;
-    if (more) p.run(A, Mk, warp, lane);
-    if (k > 0) p2.run(Q, Mk, warp, lane);
+    if (!second) {
+      block_product<NB>(A + fx, A + fy, d);
+      const double v0 = (r == c ? a : 0.0) + b * A[r * S + c] + cc * d[0];
+      const double v1 = (r == c + 1 ? a : 0.0) + b * A[r * S + c + 1] + cc * d[1];
+      put(Mk, v0, v1);
+      if (k == 0) put(Q, v0, v1);
+    }
     __syncthreads();
-    if (more) p.each(warp, lane, [&](int r, int col, double v) { both(W, r, col, v); });
-    if (k > 0) p2.each(warp, lane, [&](int r, int col, double v) { both(Q, r, col, v); });
+    if (second ? k > 0 : more) block_product<NB>(second ? Q + fx : A + fx, Mk + fy, d);
+    __syncthreads();
+    if (second ? k > 0 : more) put(second ? Q : W, d[0], d[1]);
     __syncthreads();
     if (more) {
-      p.run(W, Mk, warp, lane);
-      p.each(warp, lane, [&](int r, int col, double v) { both(A, r, col, v); });
+      if (!second) {
+        block_product<NB>(W + fx, Mk + fy, d);
+        put(A, d[0], d[1]);
+      }
       __syncthreads();
     }
   }
   double* q = P.q + (int64_t)blockIdx.x * kRows * kRows;
-  for (int e = threadIdx.x; e < kRows * kRows; e += kNsThreads) MHC_ST(q + e, Q[e / kRows * S + e % kRows] * inv);
+  for (int e = threadIdx.x; e < kRows * kRows; e += kT) MHC_ST(q + e, Q[e / kRows * S + e % kRows] * inv);
+}
+
+// The iteration on larger matrices, a cluster each.  One CTA's matrix pipe
+// needs 40 us for five steps on 80 rows at its peak (83 measured); the cluster's
+// CTAs share the rows, kSP row blocks each.  With A whole in every CTA, a strip
+// X of rows stays local under X -> X A, so a step is four of these,
+//   B = A_s A, C = B A, D = C A, E = D A:
+//   A_s' = a^2 A_s + 2ab B + (b^2 + 2ac) C + 2bc D + c^2 E,
+//   Q_s' = a Q_s + b Q_s A + c (Q_s A) A,
+// and one exchange of the new strips.  That goes through a copy in global memory
+// (the L2): a CTA's stores into the others' shared memory took 320 cycles for
+// each of them, 3,200 a step at ten CTAs.  Two warps have a block column,
+// one for each chain of products; every lane keeps its two elements of a strip
+// in registers.
+template <int NB, int kSP>
+constexpr size_t cluster_smem() {
+  return (size_t)(8 * NB + 5 * 8 * kSP) * ns_stride(NB) * sizeof(double);
+}
+template <int NB, int kSP>
+__global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_constant__ Params P) {
+  constexpr int kRows = 8 * NB, S = ns_stride(NB), kB = lower_blocks(NB), kCl = NB / kSP, kT = 64 * NB;
+  extern __shared__ __align__(16) unsigned char smem[];
+  double* A = reinterpret_cast<double*>(smem);       // this step's whole matrix
+  double* strips = A + kRows * S;
+  double *X0 = strips, *X1 = strips + 8 * kSP * S, *X2 = strips + 16 * kSP * S;   // B, C, D
+  double *Qs = strips + 24 * kSP * S, *QA = strips + 32 * kSP * S;
+  __shared__ double inv_norm;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool qside = warp >= NB;                     // this warp has the Q chain
+  const int col = qside ? warp - NB : warp;          // and this block column
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int rank = (int)cluster.block_rank(), mat = blockIdx.x / kCl;
+  const int fr = lane >> 2, fc = lane & 3;           // fragment place in a block
+  const int row0 = rank * kSP * 8;                   // the strip's first row
+  const int c = 8 * col + 2 * fc;                    // this lane's two columns
+  double* shared_a = P.exchange + (int64_t)mat * 2 * kRows * kRows;   // two copies in turn
+  auto gather = [&](int which) {                     // the others' strips; never cached in L1
+    const double2* src = reinterpret_cast<const double2*>(shared_a + which * kRows * kRows);
+    constexpr int kRowPairs = kRows / 2;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < kRows * kRowPairs; e += kT)
+      *reinterpret_cast<double2*>(A + e / kRowPairs * S + 2 * (e % kRowPairs)) = __ldcg(MHC_LDP(src + e, 16));
+  };
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  {
+    // the Gram partial sums, each block by one warp of the cluster
+    int segments;
+    const double* part = partials(P, mat, kB, segments);
+    for (int x = rank * 2 * NB + warp; x < kB; x += kCl * 2 * NB) {
+      double v0 = 0.0, v1 = 0.0;
+#pragma unroll 16
+      for (int s = 0; s < segments; ++s) {
+        const double2 v = MHC_LD(reinterpret_cast<const double2*>(part + (int64_t)s * (kB * 64) + x * 64 + 2 * lane));
+        v0 += v.x;
+        v1 += v.y;
+      }
+      int bi = 0;
+      while (lower_blocks(bi + 1) <= x) ++bi;
+      const int bj = x - lower_blocks(bi), r = 8 * bi + fr, cc = 8 * bj + 2 * fc;
+      if (bj < bi) {   // below the diagonal blocks: the mirror image too
+        MHC_ST(shared_a + cc * kRows + r, v0);
+        MHC_ST(shared_a + (cc + 1) * kRows + r, v1);
+      }
+      MHC_ST(reinterpret_cast<double2*>(shared_a + r * kRows + cc), make_double2(v0, v1));
+    }
+  }
+  cluster.sync();
+  gather(0);
+  __syncthreads();
+  if (warp == 0) {
+    const double v = inverse_norm(A, kRows, S, P.eps);
+    if (lane == 0) inv_norm = v;
+  }
+  __syncthreads();
+  const double inv = inv_norm;
+  for (int e = threadIdx.x; e < kRows * kRows; e += kT) A[e / kRows * S + e % kRows] *= inv * inv;
+  __syncthreads();
+  double as[kSP][2], q[kSP][2];   // the lane's elements: as on the A side, q on the Q side
+#pragma unroll
+  for (int s = 0; s < kSP; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) as[s][j] = A[(row0 + 8 * s + fr) * S + c + j];
+  // strip rows in X (row stride S) times this warp's block column of A
+  auto times = [&](const double* X, double (&d)[kSP][2]) {
+#pragma unroll
+    for (int s = 0; s < kSP; ++s) block_product<NB>(X + (8 * s + fr) * S + fc, A + (8 * col + fr) * S + fc, d[s]);
+  };
+  auto put = [&](double* X, const double (&d)[kSP][2]) {
+#pragma unroll
+    for (int s = 0; s < kSP; ++s)
+      *reinterpret_cast<double2*>(X + (8 * s + fr) * S + c) = make_double2(d[s][0], d[s][1]);
+  };
+  for (int k = 0; k < P.steps; ++k) {
+    const double a = P.coeffs[3 * k], b = P.coeffs[3 * k + 1], cc = P.coeffs[3 * k + 2];
+    const bool more = k + 1 < P.steps;
+    double B[kSP][2], C[kSP][2], D[kSP][2], E[kSP][2];
+    if (qside) {
+      if (k == 0) {
+        // Q = I: the new Q is the step's polynomial itself, B from the A side
+      } else {
+        times(Qs, B);        // Q A
+        put(QA, B);
+      }
+    } else if (k == 0 || more) {
+      times(A + row0 * S, B);
+      put(X0, B);
+    }
+    __syncthreads();
+    if (qside) {
+      if (k == 0) {
+#pragma unroll
+        for (int s = 0; s < kSP; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            q[s][j] = (row0 + 8 * s + fr == c + j ? a : 0.0) + b * as[s][j] + cc * X0[(8 * s + fr) * S + c + j];
+      } else {
+        times(QA, C);
+#pragma unroll
+        for (int s = 0; s < kSP; ++s)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) q[s][j] = a * q[s][j] + b * B[s][j] + cc * C[s][j];
+      }
+      put(Qs, q);            // read before the barrier above
+    } else if (more) {
+      times(X0, C);
+      put(X1, C);
+    }
+    if (!more) break;
+    __syncthreads();
+    if (!qside) {
+      times(X1, D);
+      put(X2, D);
+    }
+    __syncthreads();
+    if (!qside) {
+      times(X2, E);
+      const double ka = a * a, kb = 2 * a * b, kc = b * b + 2 * a * cc, kd = 2 * b * cc, ke = cc * cc;
+      double* dst = shared_a + ((k + 1) & 1) * kRows * kRows;
+#pragma unroll
+      for (int s = 0; s < kSP; ++s) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          as[s][j] = ka * as[s][j] + kb * B[s][j] + kc * C[s][j] + kd * D[s][j] + ke * E[s][j];
+        MHC_ST(reinterpret_cast<double2*>(dst + (row0 + 8 * s + fr) * kRows + c), make_double2(as[s][0], as[s][1]));
+      }
+    }
+    // the strips are written and A has been read; a copy is written again two
+    // steps later, behind a barrier that its readers have passed
+    cluster.sync();
+    gather((k + 1) & 1);
+    __syncthreads();
+  }
+  double* out = P.q + (int64_t)mat * kRows * kRows;
+  if (qside)
+#pragma unroll
+    for (int s = 0; s < kSP; ++s)
+      MHC_ST(reinterpret_cast<double2*>(out + (row0 + 8 * s + fr) * kRows + c),
+             make_double2(q[s][0] * inv, q[s][1] * inv));
 }
 
 // O = Q U and what is made of it: the output, or the parameter's update
@@ -436,22 +592,33 @@ __global__ void __launch_bounds__(kNsThreads) iterate_kernel(const __grid_consta
 // 4 (l / 4) .. of row 4 k + l % 4, which are its B fragments of four 8-column
 // products whose columns lie four apart; their results leave it eight
 // neighbouring columns 8 (l % 4) .. of rows l / 4 + 8 i.  So both ends are whole
-// vectors and nothing goes through shared memory but Q.
+// vectors and nothing goes through shared memory but Q and the old parameters,
+// which are fetched there (cp.async, by the lane that updates them) while the
+// products run.  The next columns' first rows are loaded before this step's
+// results are stored.
 constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
 constexpr int apply_ahead(int NB) { return NB <= 3 ? 2 * NB : 4; }   // row loads in flight
-template <int NB>
-constexpr size_t apply_smem() {
-  return (size_t)(8 * NB) * ns_stride(NB) * sizeof(double);
+// 16-byte pieces of old parameters a lane fetches: two halves of four columns a row block
+template <int NB, class TO>
+constexpr int apply_pieces() {
+  return NB * 8 * (int)sizeof(TO) / 16;
 }
-constexpr int kApplyCols = 32 * kWarps;   // columns of a CTA's step
+template <int NB, class TO, bool kStage>
+constexpr size_t apply_smem(int warps) {
+  return (size_t)(8 * NB) * ns_stride(NB) * sizeof(double) +
+         (kStage ? (size_t)warps * apply_pieces<NB, TO>() * 32 * 16 : 0);
+}
 template <int NB, class T, class TO, bool kMom, bool kVec>
 __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(const __grid_constant__ Params P,
                                                                              const __grid_constant__ Mats M) {
   constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB);
+  constexpr bool kStage = kMom && kVec;
+  constexpr int kPieces = apply_pieces<NB, TO>(), kPer = 8 * (int)sizeof(TO) / 16;   // pieces of a row block
   extern __shared__ __align__(16) unsigned char smem[];
   double* Q = reinterpret_cast<double*>(smem);   // [kRows][S]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int steps = (P.C + kApplyCols - 1) / kApplyCols;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  uint4* olds = reinterpret_cast<uint4*>(Q + kRows * S) + warp * kPieces * 32 + lane;   // [kPieces][32]
+  const int steps = (P.C + 32 * warps - 1) / (32 * warps);
   const int64_t total = (int64_t)P.mats * steps;
   const int64_t x0 = share(total, gridDim.x, blockIdx.x), x1 = share(total, gridDim.x, blockIdx.x + 1);
   float keep = 0.f, step = 0.f;
@@ -460,24 +627,58 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
     keep = 1.f - lr * P.decay;
     step = -lr * P.scale;
   }
-  int loaded = -1;
-  for (int64_t x = x1 - 1; x >= x0; --x) {
-    const int mat = (int)(x / steps);
-    const int64_t col = (x - (int64_t)mat * steps) * kApplyCols + warp * 32;
-    const T* grad = static_cast<const T*>(M.grad[mat]);
-    TO* out = static_cast<TO*>(M.out[mat]);
-    Raw4<T> g[kAhead];
-    Raw4<float> m[kAhead];
-    auto fetch = [&](int k) {
-      load4<kVec>(g[k % kAhead], grad, P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
-      if (kMom) load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
-    };
+  Raw4<T> g[kAhead];
+  Raw4<float> m[kAhead];
+  auto place = [&](int64_t x, int& mat, int64_t& col) {
+    mat = (int)(x / steps);
+    col = (x - (int64_t)mat * steps) * (32 * warps) + warp * 32;
+  };
+  auto fetch = [&](int mat, int64_t col, int k) {
+    load4<kVec>(g[k % kAhead], static_cast<const T*>(M.grad[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
+    if (kMom)
+      load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
+  };
+  int loaded = -1, mat;
+  int64_t col;
+  // from the end: what the Gram pass touched last is the likeliest to be in the L2
+  place(x1 - 1, mat, col);
+  if (x0 < x1)
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(k);
+    for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
+  for (int64_t x = x1 - 1; x >= x0; --x) {
+    place(x, mat, col);
+    TO* out = static_cast<TO*>(M.out[mat]);
+    const int64_t oc = col + 8 * (lane & 3);   // this lane's eight columns of the result
+    if constexpr (kStage) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = 8 * (i / kPer) + (lane >> 2);
+        const int64_t pc = oc + (i % kPer) * (16 / (int)sizeof(TO));
+        const TO* src = out + r * P.rs + pc;
+        // rows end on a multiple of four elements: of eight bf16 the second half may be beyond
+        const int bytes = r < P.R && pc < P.C ? (int)min((int64_t)16, (P.C - pc) * (int64_t)sizeof(TO)) : 0;
+        const uint32_t d = (uint32_t)__cvta_generic_to_shared(olds + i * 32);
+        if constexpr (sizeof(TO) == 4) {
+          const int n = bytes && MHC_CHK(src, bytes) ? bytes : 0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+        } else {   // eight-byte pieces: the rows need not be 16-byte aligned
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int n = bytes > 8 * h && MHC_CHK(src + 4 * h, 8) ? 8 : 0;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d + 8 * h), "l"(src + 4 * h), "r"(n)
+                         : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     if (mat != loaded) {   // the same for the whole CTA
+      // gradients and momenta were ready when this kernel could start; Q is
+      // not before the iteration has ended
+      cudaGridDependencySynchronize();
       __syncthreads();
       const double* q = P.q + (int64_t)mat * kRows * kRows;
-      for (int e = threadIdx.x; e < kRows * kRows; e += kThreads) Q[e / kRows * S + e % kRows] = MHC_LD(q + e);
+      for (int e = threadIdx.x; e < kRows * kRows; e += blockDim.x) Q[e / kRows * S + e % kRows] = MHC_LD(q + e);
       __syncthreads();
       loaded = mat;
     }
@@ -497,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
       }
-      if (k + kAhead < kK) fetch(k + kAhead);
+      if (k + kAhead < kK) fetch(mat, col, k + kAhead);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const double q = a[8 * i * S + 4 * k];
@@ -505,32 +706,39 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
         for (int e = 0; e < 4; ++e) dmma(acc[i][e], q, (double)f[e]);
       }
     }
-    const int64_t oc = col + 8 * (lane & 3);
-    constexpr int kBatch = NB <= 3 ? NB : 2;   // row blocks whose parameters are loaded together
+    if (x > x0) {
+      int nmat;
+      int64_t ncol;
+      place(x - 1, nmat, ncol);
 #pragma unroll
-    for (int i0 = 0; i0 < NB; i0 += kBatch) {
-      Raw4<TO> p[kBatch][2];
-      if (kMom)
+      for (int k = 0; k < kAhead; ++k) fetch(nmat, ncol, k);
+    }
+    if constexpr (kStage) asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-          if (i0 + i < NB)
+    for (int i = 0; i < NB; ++i) {
+      const int r = 8 * i + (lane >> 2);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              load4<kVec>(p[i][j], static_cast<const TO*>(out), P, 8 * (i0 + i) + (lane >> 2), oc + 4 * j);
+      for (int j = 0; j < 2; ++j) {
+        float o[4], old[4];
+        if constexpr (kStage) {
+          Raw4<TO> raw;
+          if constexpr (sizeof(TO) == 4)
+            raw.v = *reinterpret_cast<const float4*>(olds + (2 * i + j) * 32);
+          else
+            raw.v = reinterpret_cast<const uint2*>(olds + i * 32)[j];
+          raw.unpack(old);
+        } else if constexpr (kMom) {
+          Raw4<TO> raw;
+          load4<kVec>(raw, static_cast<const TO*>(out), P, r, oc + 4 * j);
+          raw.unpack(old);
+        }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (i0 + i < NB)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float o[4], old[4];
-            if (kMom) p[i][j].unpack(old);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = (float)acc[i0 + i][e][j];
-              o[e] = kMom ? fmaf(keep, old[e], step * v) : v;
-            }
-            store4<kVec>(out, P, 8 * (i0 + i) + (lane >> 2), oc + 4 * j, o);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float v = (float)acc[i][e][j];
+          o[e] = kMom ? fmaf(keep, old[e], step * v) : v;
+        }
+        store4<kVec>(out, P, r, oc + 4 * j, o);
+      }
     }
   }
 }
