@@ -595,9 +595,13 @@ __global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_c
 // vectors and nothing goes through shared memory but Q and the old parameters,
 // which are fetched there (cp.async, by the lane that updates them) while the
 // products run.  The next columns' first rows are loaded before this step's
-// results are stored.
+// results are stored.  With few rows all of a step's loads are in registers at
+// once instead, and other warps' work covers them.
 constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
 constexpr int apply_ahead(int NB) { return NB <= 3 ? 2 * NB : 4; }   // row loads in flight
+// Old parameters go through shared memory where the registers are full of sums
+// (24 rows: 76 us with them loaded behind the products, 82 through shared memory).
+constexpr bool apply_stages(int NB, bool mom, bool vec) { return NB > 3 && mom && vec; }
 // 16-byte pieces of old parameters a lane fetches: two halves of four columns a row block
 template <int NB, class TO>
 constexpr int apply_pieces() {
@@ -606,13 +610,13 @@ constexpr int apply_pieces() {
 template <int NB, class TO, bool kStage>
 constexpr size_t apply_smem(int warps) {
   return (size_t)(8 * NB) * ns_stride(NB) * sizeof(double) +
-         (kStage ? (size_t)warps * apply_pieces<NB, TO>() * 32 * 16 : 0);
+         (kStage && NB > 3 ? (size_t)warps * apply_pieces<NB, TO>() * 32 * 16 : 0);
 }
 template <int NB, class T, class TO, bool kMom, bool kVec>
 __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(const __grid_constant__ Params P,
                                                                              const __grid_constant__ Mats M) {
   constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB);
-  constexpr bool kStage = kMom && kVec;
+  constexpr bool kStage = apply_stages(NB, kMom, kVec);
   constexpr int kPieces = apply_pieces<NB, TO>(), kPer = 8 * (int)sizeof(TO) / 16;   // pieces of a row block
   extern __shared__ __align__(16) unsigned char smem[];
   double* Q = reinterpret_cast<double*>(smem);   // [kRows][S]
@@ -642,13 +646,16 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
   int64_t col;
   // from the end: what the Gram pass touched last is the likeliest to be in the L2
   place(x1 - 1, mat, col);
-  if (x0 < x1)
+  if (kStage && x0 < x1)
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
   for (int64_t x = x1 - 1; x >= x0; --x) {
     place(x, mat, col);
     TO* out = static_cast<TO*>(M.out[mat]);
     const int64_t oc = col + 8 * (lane & 3);   // this lane's eight columns of the result
+    if constexpr (!kStage)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
     if constexpr (kStage) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
@@ -706,39 +713,44 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
         for (int e = 0; e < 4; ++e) dmma(acc[i][e], q, (double)f[e]);
       }
     }
-    if (x > x0) {
-      int nmat;
-      int64_t ncol;
-      place(x - 1, nmat, ncol);
+    if constexpr (kStage) {
+      if (x > x0) {
+        int nmat;
+        int64_t ncol;
+        place(x - 1, nmat, ncol);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) fetch(nmat, ncol, k);
-    }
-    if constexpr (kStage) asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int r = 8 * i + (lane >> 2);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float o[4], old[4];
-        if constexpr (kStage) {
-          Raw4<TO> raw;
-          if constexpr (sizeof(TO) == 4)
-            raw.v = *reinterpret_cast<const float4*>(olds + (2 * i + j) * 32);
-          else
-            raw.v = reinterpret_cast<const uint2*>(olds + i * 32)[j];
-          raw.unpack(old);
-        } else if constexpr (kMom) {
-          Raw4<TO> raw;
-          load4<kVec>(raw, static_cast<const TO*>(out), P, r, oc + 4 * j);
-          raw.unpack(old);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = (float)acc[i][e][j];
-          o[e] = kMom ? fmaf(keep, old[e], step * v) : v;
-        }
-        store4<kVec>(out, P, r, oc + 4 * j, o);
+        for (int k = 0; k < kAhead; ++k) fetch(nmat, ncol, k);
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    constexpr int kBatch = NB <= 3 && kVec ? NB : 1;   // row blocks whose parameters are loaded together
+#pragma unroll
+    for (int b = 0; b < NB; b += kBatch) {
+      Raw4<TO> old[kBatch][2];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (kStage && sizeof(TO) == 4)
+            old[i][j].v = *reinterpret_cast<const float4*>(olds + (2 * (b + i) + j) * 32);
+          else if constexpr (kStage)
+            old[i][j].v = reinterpret_cast<const uint2*>(olds + (b + i) * 32)[j];
+          else if constexpr (kMom)
+            load4<kVec>(old[i][j], static_cast<const TO*>(out), P, 8 * (b + i) + (lane >> 2), oc + 4 * j);
+        }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float o[4], p[4];
+          if constexpr (kMom) old[i][j].unpack(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = (float)acc[b + i][e][j];
+            o[e] = kMom ? fmaf(keep, p[e], step * v) : v;
+          }
+          store4<kVec>(out, P, 8 * (b + i) + (lane >> 2), oc + 4 * j, o);
+        }
     }
   }
 }
