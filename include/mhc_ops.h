@@ -441,7 +441,7 @@ typedef struct mhc_muon_args {
 } mhc_muon_args;
 
 /* Workspace bytes of mhc_orthogonalize and mhc_muon_step for these sizes on
- * the current device. */
+ * the current device (0 for small matrices, which need none). */
 MHC_API int mhc_ortho_workspace_size(int64_t count, int32_t rows, int32_t cols, size_t* bytes);
 MHC_API int mhc_orthogonalize(const mhc_ortho_args* args, void* stream);
 MHC_API int mhc_muon_step(const mhc_muon_args* args, void* stream);

@@ -1256,6 +1256,7 @@ int rope_dispatch(const mhc_qk_args* a, const rope::Params& p, const RopePlan& r
 // ------------------------------------------------------- updates of phi
 struct OrthoPlan {
   int R, C, NB, chunks, gram_ctas, segments, apply_ctas, apply_warps, mats;   // mats: matrices of one launch
+  bool fused;                                                                 // one launch, no workspace
   int64_t rs, cs;
   size_t q_off, exchange_off, total;
 };
@@ -1271,6 +1272,8 @@ OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   p.cs = tall ? cols : 1;
   p.NB = ortho::row_blocks(p.R);
   p.mats = (int)std::min<int64_t>(count, ortho::kMaxMats);
+  p.fused = ortho::fused_fits(p.NB, p.C);
+  if (p.fused) return p;
   const int kc = ortho::chunk_cols(p.NB);
   p.chunks = (p.C + kc - 1) / kc;
   // As many CTAs as the device holds, but a limit to a matrix's partial sums,
@@ -1367,6 +1370,16 @@ int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, cudaStre
 template <int NB, class T, class TO, bool kMom>
 int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats& m, bool vec, int sms,
                  cudaStream_t s) {
+  if constexpr (NB <= ortho::kFusedBlocks) {
+    if (pl.fused) {
+      auto fused = vec ? ortho::fused_kernel<NB, T, TO, kMom, true> : ortho::fused_kernel<NB, T, TO, kMom, false>;
+      const int smem = (int)ortho::fused_smem<NB>(pl.C);
+      if (smem > kDefaultSmem)
+        MHC_CUDA_TRY(cudaFuncSetAttribute(fused, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      fused<<<pl.mats, ortho::kFusedThreads, smem, s>>>(p, m);
+      return after_launch();
+    }
+  }
   constexpr int gs = (int)ortho::gram_smem<NB>();
   const int as = (int)(vec && kMom ? ortho::apply_smem<NB, TO, true>(pl.apply_warps)
                                    : ortho::apply_smem<NB, TO, false>(pl.apply_warps));
@@ -1509,9 +1522,11 @@ int ortho_check_lists(const OrthoLists& l, int64_t count, int rows, int cols, bo
       return MHC_ERR_MISALIGNED;
   }
   if (int st = ortho_overlap(l, count, (size_t)rows * cols, same)) return st;
+  const size_t need = ortho_workspace(count, rows, cols, sms);
+  if (need == 0) return MHC_OK;
   if (!workspace) return MHC_ERR_NULL_POINTER;
   if (!aligned(workspace, kWsAlign)) return MHC_ERR_MISALIGNED;
-  if (workspace_bytes < ortho_workspace(count, rows, cols, sms)) return MHC_ERR_WORKSPACE_TOO_SMALL;
+  if (workspace_bytes < need) return MHC_ERR_WORKSPACE_TOO_SMALL;
   return MHC_OK;
 }
 

@@ -128,23 +128,26 @@ __device__ __forceinline__ void st1(T* p, float v) {
   if constexpr (std::is_same_v<T, float>) MHC_ST(p, v);
   else MHC_ST(p, f32_to_bf16_bits(v));
 }
-// Elements (r, c .. c + 3); zeros beyond the matrix.  kVec: rows of cs = 1 that
-// start on a multiple of four elements and have a multiple of four of them.
+// Elements (r, c + j * gap), j = 0 .. 3; zeros beyond the matrix.  kVec: rows of
+// cs = 1 that start on a multiple of four elements and have a multiple of four
+// of them, gap 1.  Element by element a wider gap lets neighbouring lanes take
+// neighbouring columns.
 template <bool kVec, class T>
-__device__ __forceinline__ void load4(Raw4<T>& raw, const T* base, const Params& P, int r, int64_t c) {
+__device__ __forceinline__ void load4(Raw4<T>& raw, const T* base, const Params& P, int r, int64_t c, int gap = 1) {
   raw.v = {};
   if constexpr (kVec) {
     if (r < P.R && c < P.C) raw.v = MHC_LD(reinterpret_cast<const typename Raw4<T>::V*>(base + r * P.rs + c));
   } else {
+    const T* p = base + r * P.rs + c * P.cs;
+    const int64_t d = gap * P.cs;
     float f[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      f[j] = r < P.R && c + j < P.C ? ld1(base + r * P.rs + (c + j) * P.cs) : 0.f;
+    for (int j = 0; j < 4; ++j) f[j] = r < P.R && c + j * gap < P.C ? ld1(p + j * d) : 0.f;
     raw.pack(f);
   }
 }
 template <bool kVec, class T>
-__device__ __forceinline__ void store4(T* base, const Params& P, int r, int64_t c, const float (&f)[4]) {
+__device__ __forceinline__ void store4(T* base, const Params& P, int r, int64_t c, const float (&f)[4], int gap = 1) {
   if constexpr (kVec) {
     if (r < P.R && c < P.C) {
       Raw4<T> raw;
@@ -152,9 +155,11 @@ __device__ __forceinline__ void store4(T* base, const Params& P, int r, int64_t 
       MHC_ST(reinterpret_cast<typename Raw4<T>::V*>(base + r * P.rs + c), raw.v);
     }
   } else {
+    T* p = base + r * P.rs + c * P.cs;
+    const int64_t d = gap * P.cs;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (r < P.R && c + j < P.C) st1(base + r * P.rs + (c + j) * P.cs, f[j]);
+      if (r < P.R && c + j * gap < P.C) st1(p + j * d, f[j]);
   }
 }
 
@@ -218,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
   constexpr int kRows = 8 * NB, KC = chunk_cols(NB), kStride = KC + 4, kB = lower_blocks(NB);
   constexpr int kRoles = gram_roles(NB), kColWarps = kWarps / kRoles, kWarpCols = KC / kColWarps;
   constexpr int kPer = kRows * (KC / 4) / kThreads;   // 4-element pieces of a chunk per thread
+  constexpr int kGap = kVec ? 1 : KC / 4;             // columns between a piece's elements
   static_assert(kRows * (KC / 4) % kThreads == 0 && kWarpCols % 4 == 0, "chunk split");
   extern __shared__ __align__(16) unsigned char smem[];
   float* tile = reinterpret_cast<float*>(smem);       // two of [kRows][kStride]
@@ -232,9 +238,9 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
     const int64_t col = (x - (int64_t)mat * P.chunks) * KC;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * 4;
-      load4<kVec>(g[i], static_cast<const T*>(M.grad[mat]), P, r, col + c);
-      if (kMom) load4<kVec>(m[i], static_cast<const float*>(M.mom[mat]), P, r, col + c);
+      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * (kVec ? 4 : 1);
+      load4<kVec>(g[i], static_cast<const T*>(M.grad[mat]), P, r, col + c, kGap);
+      if (kMom) load4<kVec>(m[i], static_cast<const float*>(M.mom[mat]), P, r, col + c, kGap);
     }
   };
   auto stage = [&](int64_t x, float* dst) {
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
     const int64_t col = (x - (int64_t)mat * P.chunks) * KC;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * 4;
+      const int e = threadIdx.x + i * kThreads, r = e / (KC / 4), c = (e % (KC / 4)) * (kVec ? 4 : 1);
       float f[4];
       g[i].unpack(f);
       if (kMom) {
@@ -253,9 +259,14 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
           m1[j] = new_momentum(m1[j], f[j], P.momentum);
           f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
         }
-        store4<kVec>(M.mom[mat], P, r, col + c, m1);
+        store4<kVec>(M.mom[mat], P, r, col + c, m1, kGap);
       }
-      *reinterpret_cast<float4*>(dst + r * kStride + c) = make_float4(f[0], f[1], f[2], f[3]);
+      if constexpr (kVec) {
+        *reinterpret_cast<float4*>(dst + r * kStride + c) = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dst[r * kStride + c + j * kGap] = f[j];
+      }
     }
   };
 
@@ -357,74 +368,210 @@ template <int NB>
 constexpr size_t small_smem() {
   return (size_t)4 * (8 * NB) * ns_stride(NB) * sizeof(double);
 }
+// The place of a warp and lane in it; warps past the two sets have none.
+template <int NB>
+struct SmallPlace {
+  static constexpr int kB = lower_blocks(NB), S = ns_stride(NB);
+  bool first, second;   // this warp has a block of the first or of the second product
+  int x, r, c, fx, fy;  // its block, this lane's two results (r, c), (r, c + 1), fragment places
+  __device__ __forceinline__ SmallPlace() {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    first = warp < kB;
+    second = warp >= kB && warp < 2 * kB;
+    x = second ? warp - kB : first ? warp : 0;
+    int bi = 0;
+    while (lower_blocks(bi + 1) <= x) ++bi;
+    const int bj = x - lower_blocks(bi);
+    r = 8 * bi + (lane >> 2);
+    c = 8 * bj + 2 * (lane & 3);
+    fx = (8 * bi + (lane >> 2)) * S + (lane & 3);
+    fy = (8 * bj + (lane >> 2)) * S + (lane & 3);
+  }
+  __device__ __forceinline__ void put(double* X, double v0, double v1) const {   // a result and its mirror image
+    X[r * S + c] = v0;
+    X[r * S + c + 1] = v1;
+    X[c * S + r] = v0;
+    X[(c + 1) * S + r] = v1;
+  }
+};
+// From the Gram matrix in A (all of it, behind a barrier) to Q, by a whole CTA;
+// returns 1 / (|U|_F + eps), which Q lacks.  Q is behind a barrier.
+template <int NB>
+__device__ __forceinline__ double iterate_small(const Params& P, const SmallPlace<NB>& pl, double* A, double* Mk,
+                                                double* W, double* Q, double* shared_inv) {
+  constexpr int kRows = 8 * NB, S = ns_stride(NB);
+  if (threadIdx.x < 32) {
+    const double v = inverse_norm(A, kRows, S, P.eps);
+    if (threadIdx.x == 0) *shared_inv = v;
+  }
+  __syncthreads();
+  const double inv = *shared_inv;
+  for (int e = threadIdx.x; e < kRows * kRows; e += blockDim.x) A[e / kRows * S + e % kRows] *= inv * inv;
+  __syncthreads();
+  double d[2];
+  for (int k = 0; k < P.steps; ++k) {
+    const double a = P.coeffs[3 * k], b = P.coeffs[3 * k + 1], cc = P.coeffs[3 * k + 2];
+    const bool more = k + 1 < P.steps;
+    if (pl.first) {
+      block_product<NB>(A + pl.fx, A + pl.fy, d);
+      const int at = pl.r * S + pl.c;
+      const double v0 = (pl.r == pl.c ? a : 0.0) + b * A[at] + cc * d[0];
+      const double v1 = (pl.r == pl.c + 1 ? a : 0.0) + b * A[at + 1] + cc * d[1];
+      pl.put(Mk, v0, v1);
+      if (k == 0) pl.put(Q, v0, v1);
+    }
+    __syncthreads();
+    const bool work = (pl.first && more) || (pl.second && k > 0);
+    if (work) block_product<NB>(pl.second ? Q + pl.fx : A + pl.fx, Mk + pl.fy, d);
+    __syncthreads();
+    if (work) pl.put(pl.second ? Q : W, d[0], d[1]);
+    __syncthreads();
+    if (more) {
+      if (pl.first) {
+        block_product<NB>(W + pl.fx, Mk + pl.fy, d);
+        pl.put(A, d[0], d[1]);
+      }
+      __syncthreads();
+    }
+  }
+  return inv;
+}
 template <int NB>
 __global__ void __launch_bounds__(32 * small_warps(NB)) iterate_small_kernel(const __grid_constant__ Params P) {
   constexpr int kRows = 8 * NB, S = ns_stride(NB), kB = lower_blocks(NB), kT = 32 * small_warps(NB);
   extern __shared__ __align__(16) unsigned char smem[];
   double* A = reinterpret_cast<double*>(smem);
   double *Mk = A + kRows * S, *W = Mk + kRows * S, *Q = W + kRows * S;
-  __shared__ double inv_norm;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool second = warp >= kB;
-  const int x = second ? warp - kB : warp;
-  int bi = 0;
-  while (lower_blocks(bi + 1) <= x) ++bi;
-  const int bj = x - lower_blocks(bi);
-  const int r = 8 * bi + (lane >> 2), c = 8 * bj + 2 * (lane & 3);           // this lane's two results
-  const int fx = (8 * bi + (lane >> 2)) * S + (lane & 3), fy = (8 * bj + (lane >> 2)) * S + (lane & 3);
-  auto put = [&](double* X, double v0, double v1) {   // a result and its mirror image
-    X[r * S + c] = v0;
-    X[r * S + c + 1] = v1;
-    X[c * S + r] = v0;
-    X[(c + 1) * S + r] = v1;
-  };
+  __shared__ double shared_inv;
+  const SmallPlace<NB> pl;
+  const int odd = pl.second ? 1 : 0;   // first warps add the even elements of their block, second ones the odd
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   int segments;
-  const double* part = partials(P, blockIdx.x, kB, segments) + x * 64 + 2 * lane + (second ? 1 : 0);
-  {
-    double v = 0.0;   // first warps: the even elements of their block, second ones the odd
+  const double* part = partials(P, blockIdx.x, kB, segments) + pl.x * 64 + 2 * (threadIdx.x & 31) + odd;
+  double v = 0.0;
 #pragma unroll 16
-    for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64));
-    const int cc = c + (second ? 1 : 0);
-    A[r * S + cc] = v;
-    A[cc * S + r] = v;
-  }
+  for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64));
+  A[pl.r * S + pl.c + odd] = v;
+  A[(pl.c + odd) * S + pl.r] = v;
   __syncthreads();
-  if (warp == 0) {
-    const double v = inverse_norm(A, kRows, S, P.eps);
-    if (lane == 0) inv_norm = v;
-  }
-  __syncthreads();
-  const double inv = inv_norm;
-  for (int e = threadIdx.x; e < kRows * kRows; e += kT) A[e / kRows * S + e % kRows] *= inv * inv;
-  __syncthreads();
-  double d[2];
-  for (int k = 0; k < P.steps; ++k) {
-    const double a = P.coeffs[3 * k], b = P.coeffs[3 * k + 1], cc = P.coeffs[3 * k + 2];
-    const bool more = k + 1 < P.steps;
-    if (!second) {
-      block_product<NB>(A + fx, A + fy, d);
-      const double v0 = (r == c ? a : 0.0) + b * A[r * S + c] + cc * d[0];
-      const double v1 = (r == c + 1 ? a : 0.0) + b * A[r * S + c + 1] + cc * d[1];
-      put(Mk, v0, v1);
-      if (k == 0) put(Q, v0, v1);
-    }
-    __syncthreads();
-    if (second ? k > 0 : more) block_product<NB>(second ? Q + fx : A + fx, Mk + fy, d);
-    __syncthreads();
-    if (second ? k > 0 : more) put(second ? Q : W, d[0], d[1]);
-    __syncthreads();
-    if (more) {
-      if (!second) {
-        block_product<NB>(W + fx, Mk + fy, d);
-        put(A, d[0], d[1]);
-      }
-      __syncthreads();
-    }
-  }
+  const double inv = iterate_small<NB>(P, pl, A, Mk, W, Q, &shared_inv);
   double* q = P.q + (int64_t)blockIdx.x * kRows * kRows;
   for (int e = threadIdx.x; e < kRows * kRows; e += kT) MHC_ST(q + e, Q[e / kRows * S + e % kRows] * inv);
+}
+
+// Small matrices whole in one launch, a CTA each: the matrix stays in shared
+// memory between the Gram product, the iteration and the application.  One CTA's
+// matrix pipe takes about 4 cycles a product, so the limit is 3,000 of them,
+// some 6 us, about what three kernels cost in launches and starts alone.
+constexpr int kFusedBlocks = 3;
+constexpr int kFusedThreads = 384;   // 12 warps: 24 rows' iteration needs as many
+constexpr int kFusedWarps = kFusedThreads / 32;
+__host__ __device__ constexpr int fused_stride(int C) { return (C + 31) / 32 * 32 + 4; }
+inline bool fused_fits(int NB, int C) {
+  return NB <= kFusedBlocks && (int64_t)(lower_blocks(NB) + NB * NB) * C <= 4 * 3000 &&
+         (int64_t)8 * NB * fused_stride(C) * 4 <= 128 * 1024;
+}
+template <int NB>
+size_t fused_smem(int C) {
+  return small_smem<NB>() + (size_t)kFusedWarps * lower_blocks(NB) * 64 * sizeof(double) +
+         (size_t)8 * NB * fused_stride(C) * sizeof(float);
+}
+template <int NB, class T, class TO, bool kMom, bool kVec>
+__global__ void __launch_bounds__(kFusedThreads) fused_kernel(const __grid_constant__ Params P,
+                                                              const __grid_constant__ Mats M) {
+  constexpr int kRows = 8 * NB, S = ns_stride(NB), kB = lower_blocks(NB);
+  extern __shared__ __align__(16) unsigned char smem[];
+  double* A = reinterpret_cast<double*>(smem);
+  double *Mk = A + kRows * S, *W = Mk + kRows * S, *Q = W + kRows * S;
+  double* sums = Q + kRows * S;                                              // [kFusedWarps][kB][64]
+  float* U = reinterpret_cast<float*>(sums + kFusedWarps * kB * 64);         // [kRows][stride]
+  __shared__ double shared_inv;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, stride = fused_stride(P.C), width = stride - 4;
+  const T* g = static_cast<const T*>(M.grad[blockIdx.x]);
+  float* mom = kMom ? M.mom[blockIdx.x] : nullptr;
+  TO* out = static_cast<TO*>(M.out[blockIdx.x]);
+  const int quarter = width / 4, gap = kVec ? 1 : quarter;
+  for (int e = threadIdx.x; e < kRows * quarter; e += kFusedThreads) {
+    const int r = e / quarter, c = (e % quarter) * (kVec ? 4 : 1);
+    Raw4<T> raw;
+    load4<kVec>(raw, g, P, r, c, gap);
+    float f[4];
+    raw.unpack(f);
+    if constexpr (kMom) {
+      Raw4<float> rm;
+      load4<kVec>(rm, static_cast<const float*>(mom), P, r, c, gap);
+      float m1[4];
+      rm.unpack(m1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m1[j] = new_momentum(m1[j], f[j], P.momentum);
+        f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
+      }
+      store4<kVec>(mom, P, r, c, m1, gap);
+    }
+    if constexpr (kVec) {
+      *reinterpret_cast<float4*>(U + r * stride + c) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) U[r * stride + c + j * gap] = f[j];
+    }
+  }
+  __syncthreads();
+  {
+    Gram<0, NB> gram;
+    gram.clear();
+    // every warp eight columns at a time
+    for (int c = warp * 8; c < width; c += kFusedWarps * 8) gram.run(U + c, stride, 8, lane);
+    gram.store(sums + warp * kB * 64, lane);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < kB * 64; e += kFusedThreads) {
+    double v = 0.0;
+#pragma unroll
+    for (int w = 0; w < kFusedWarps; ++w) v += sums[w * kB * 64 + e];
+    int bi = 0;
+    while (lower_blocks(bi + 1) <= e / 64) ++bi;
+    const int l = (e & 63) >> 1, r = 8 * bi + (l >> 2), c = 8 * (e / 64 - lower_blocks(bi)) + 2 * (l & 3) + (e & 1);
+    A[r * S + c] = v;
+    A[c * S + r] = v;
+  }
+  __syncthreads();
+  const SmallPlace<NB> pl;
+  const double inv = iterate_small<NB>(P, pl, A, Mk, W, Q, &shared_inv);
+  for (int e = threadIdx.x; e < kRows * kRows; e += kFusedThreads) Q[e / kRows * S + e % kRows] *= inv;
+  __syncthreads();
+  float keep = 0.f, step = 0.f;
+  if (kMom) {
+    const float lr = P.lr_dev ? MHC_LDG(P.lr_dev) : P.lr;
+    keep = 1.f - lr * P.decay;
+    step = -lr * P.scale;
+  }
+  // a warp eight columns at a time: B fragments are U[4 k + lane % 4][c + lane / 4],
+  // results the neighbouring columns c + 2 (lane % 4) and the next of rows lane / 4 + 8 i
+  for (int c = warp * 8; c < P.C; c += kFusedWarps * 8) {
+    double acc[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[i][0] = acc[i][1] = 0.0;
+#pragma unroll
+    for (int k = 0; k < 2 * NB; ++k) {
+      const double f = (double)U[(4 * k + (lane & 3)) * stride + c + (lane >> 2)];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) dmma(acc[i], Q[(8 * i + (lane >> 2)) * S + 4 * k + (lane & 3)], f);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 8 * i + (lane >> 2);
+        const int64_t oc = c + 2 * (lane & 3) + j;
+        if (r < P.R && oc < P.C) {
+          TO* o = out + r * P.rs + oc * P.cs;
+          const float v = (float)acc[i][j];
+          st1(o, kMom ? fmaf(keep, ld1(static_cast<const TO*>(o)), step * v) : v);
+        }
+      }
+  }
 }
 
 // The iteration on larger matrices, a cluster each.  One CTA's matrix pipe
@@ -592,7 +739,8 @@ __global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_c
 // 4 (l / 4) .. of row 4 k + l % 4, which are its B fragments of four 8-column
 // products whose columns lie four apart; their results leave it eight
 // neighbouring columns 8 (l % 4) .. of rows l / 4 + 8 i.  So both ends are whole
-// vectors and nothing goes through shared memory but Q and the old parameters,
+// vectors (element by element the columns of a product lie side by side instead,
+// for the lanes' sake) and nothing goes through shared memory but Q and the old parameters,
 // which are fetched there (cp.async, by the lane that updates them) while the
 // products run.  The next columns' first rows are loaded before this step's
 // results are stored.  With few rows all of a step's loads are in registers at
@@ -617,6 +765,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
                                                                              const __grid_constant__ Mats M) {
   constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB);
   constexpr bool kStage = apply_stages(NB, kMom, kVec);
+  constexpr int kGap = kVec ? 1 : 8, kHalf = kVec ? 4 : 1;
   constexpr int kPieces = apply_pieces<NB, TO>(), kPer = 8 * (int)sizeof(TO) / 16;   // pieces of a row block
   extern __shared__ __align__(16) unsigned char smem[];
   double* Q = reinterpret_cast<double*>(smem);   // [kRows][S]
@@ -638,9 +787,9 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
     col = (x - (int64_t)mat * steps) * (32 * warps) + warp * 32;
   };
   auto fetch = [&](int mat, int64_t col, int k) {
-    load4<kVec>(g[k % kAhead], static_cast<const T*>(M.grad[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
-    if (kMom)
-      load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), col + 4 * (lane >> 2));
+    const int64_t c = col + (kVec ? 4 : 1) * (lane >> 2);
+    load4<kVec>(g[k % kAhead], static_cast<const T*>(M.grad[mat]), P, 4 * k + (lane & 3), c, kGap);
+    if (kMom) load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), c, kGap);
   };
   int loaded = -1, mat;
   int64_t col;
@@ -652,7 +801,8 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
   for (int64_t x = x1 - 1; x >= x0; --x) {
     place(x, mat, col);
     TO* out = static_cast<TO*>(M.out[mat]);
-    const int64_t oc = col + 8 * (lane & 3);   // this lane's eight columns of the result
+    // this lane's eight columns of the result: half j at oc + kHalf * j, kGap apart
+    const int64_t oc = col + (kVec ? 8 : 2) * (lane & 3);
     if constexpr (!kStage)
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
@@ -736,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
           else if constexpr (kStage)
             old[i][j].v = reinterpret_cast<const uint2*>(olds + (b + i) * 32)[j];
           else if constexpr (kMom)
-            load4<kVec>(old[i][j], static_cast<const TO*>(out), P, 8 * (b + i) + (lane >> 2), oc + 4 * j);
+            load4<kVec>(old[i][j], static_cast<const TO*>(out), P, 8 * (b + i) + (lane >> 2), oc + kHalf * j, kGap);
         }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
@@ -749,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
             const float v = (float)acc[b + i][e][j];
             o[e] = kMom ? fmaf(keep, p[e], step * v) : v;
           }
-          store4<kVec>(out, P, 8 * (b + i) + (lane >> 2), oc + 4 * j, o);
+          store4<kVec>(out, P, 8 * (b + i) + (lane >> 2), oc + kHalf * j, o, kGap);
         }
     }
   }
