@@ -1277,10 +1277,10 @@ OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   const int kc = ortho::chunk_cols(p.NB);
   p.chunks = (p.C + kc - 1) / kc;
   // As many CTAs as the device holds, but a limit to a matrix's partial sums,
-  // which one CTA adds before the iteration (96 where a cluster shares that).
+  // which are added before the iteration (by a thread an element, or a cluster).
   const int64_t all = (int64_t)p.mats * p.chunks;
   p.gram_ctas = (int)std::min<int64_t>({all, (int64_t)sms * ortho::gram_occupancy(p.NB),
-                                        (int64_t)(p.NB <= ortho::kSmallBlocks ? 32 : 96) * p.mats});
+                                        (int64_t)(p.NB <= 3 ? 32 : p.NB <= ortho::kSmallBlocks ? 64 : 96) * p.mats});
   // A matrix's chunks lie in at most this many shares: a share has at least
   // all / gram_ctas of them, and one more may begin or end inside the matrix.
   const int64_t least = all / p.gram_ctas;

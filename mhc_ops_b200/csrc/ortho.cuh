@@ -746,7 +746,8 @@ __global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_c
 // results are stored.  With few rows all of a step's loads are in registers at
 // once instead, and other warps' work covers them.
 constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
-constexpr int apply_ahead(int NB) { return NB <= 3 ? 2 * NB : 4; }   // row loads in flight
+// row loads in flight; element by element they are all that hides their latency
+constexpr int apply_ahead(int NB, bool vec) { return NB <= 3 || (!vec && NB == 5) ? 2 * NB : !vec && NB == 6 ? 6 : 4; }
 // Old parameters go through shared memory where the registers are full of sums
 // (24 rows: 76 us with them loaded behind the products, 82 through shared memory).
 constexpr bool apply_stages(int NB, bool mom, bool vec) { return NB > 3 && mom && vec; }
@@ -763,7 +764,7 @@ constexpr size_t apply_smem(int warps) {
 template <int NB, class T, class TO, bool kMom, bool kVec>
 __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(const __grid_constant__ Params P,
                                                                              const __grid_constant__ Mats M) {
-  constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB);
+  constexpr int kRows = 8 * NB, S = ns_stride(NB), kK = 2 * NB, kAhead = apply_ahead(NB, kVec);
   constexpr bool kStage = apply_stages(NB, kMom, kVec);
   constexpr int kGap = kVec ? 1 : 8, kHalf = kVec ? 4 : 1;
   constexpr int kPieces = apply_pieces<NB, TO>(), kPer = 8 * (int)sizeof(TO) / 16;   // pieces of a row block

@@ -582,10 +582,13 @@ int32_t check_coeffs(at::ArrayRef<double> coeffs, double eps) {
   return (int32_t)(coeffs.size() / 3);
 }
 
-at::Tensor ortho_workspace(const Mats& m, size_t* nbytes) {
+at::Tensor ortho_workspace(const Mats& m, size_t* nbytes, void** ptr) {
   check_status(mhc_ortho_workspace_size((int64_t)m.ptrs.size(), (int32_t)m.rows, (int32_t)m.cols, nbytes),
                "mhc_ortho_workspace_size");
-  return scratch(*nbytes, m.dev);
+  at::Tensor ws;
+  if (*nbytes > 0) ws = scratch(*nbytes, m.dev);
+  *ptr = ws.defined() ? ws.data_ptr() : nullptr;
+  return ws;
 }
 
 void check_sizes(const Mats& m) {
@@ -613,7 +616,7 @@ std::vector<at::Tensor> orthogonalize_cuda(at::TensorList g, at::ArrayRef<double
   std::vector<void*> dst(m.ptrs.size());
   const int64_t step = m.rows * m.cols * (int64_t)stack.element_size();
   for (int64_t i = 0; i < count; ++i) dst[i] = static_cast<char*>(stack.data_ptr()) + i * step;
-  const at::Tensor ws = ortho_workspace(m, &a.workspace_bytes);
+  const at::Tensor ws = ortho_workspace(m, &a.workspace_bytes, &a.workspace);
   a.in = m.ptrs.data();
   a.out = dst.data();
   a.count = count;
@@ -622,7 +625,6 @@ std::vector<at::Tensor> orthogonalize_cuda(at::TensorList g, at::ArrayRef<double
   a.dtype = m.dtype;
   a.coeffs = coeffs.data();
   a.eps = eps;
-  a.workspace = ws.data_ptr();
   check_status(mhc_orthogonalize(&a, at::cuda::getCurrentCUDAStream().stream()), "mhc::orthogonalize");
   return out;
 }
@@ -649,7 +651,7 @@ void muon_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList 
                       "lr must be a number or a one-element float32 tensor on ", p.dev);
     a.lr_device = lr_tensor->data_ptr<float>();
   }
-  const at::Tensor ws = ortho_workspace(p, &a.workspace_bytes);
+  const at::Tensor ws = ortho_workspace(p, &a.workspace_bytes, &a.workspace);
   a.params = p.ptrs.data();
   a.grads = g.ptrs.data();
   a.momenta = reinterpret_cast<float* const*>(m.ptrs.data());
@@ -665,7 +667,6 @@ void muon_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList 
   a.weight_decay = (float)weight_decay;
   a.scale = (float)scale;
   a.lr = (float)lr;
-  a.workspace = ws.data_ptr();
   check_status(mhc_muon_step(&a, at::cuda::getCurrentCUDAStream().stream()), "mhc::muon_step_");
   // autograd has to see that these were written
   for (const at::Tensor& t : params)
