@@ -431,7 +431,7 @@ typedef struct mhc_muon_args {
   int32_t steps;
   const double* coeffs;
   double eps;
-  float momentum;
+  double momentum;             /* mu; 1 - mu is taken before either is rounded to 32 bits */
   float weight_decay;
   float scale;
   float lr;

@@ -118,7 +118,7 @@ class MuonArgs(ctypes.Structure):
         ("params", _c_void_p), ("grads", _c_void_p), ("momenta", _c_void_p), ("count", ctypes.c_int64),
         ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
         ("grad_dtype", ctypes.c_int32), ("nesterov", ctypes.c_int32), ("steps", ctypes.c_int32),
-        ("coeffs", _c_void_p), ("eps", ctypes.c_double), ("momentum", ctypes.c_float),
+        ("coeffs", _c_void_p), ("eps", ctypes.c_double), ("momentum", ctypes.c_double),
         ("weight_decay", ctypes.c_float), ("scale", ctypes.c_float), ("lr", ctypes.c_float), ("lr_device", _c_void_p),
         ("workspace", _c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]

@@ -2129,7 +2129,8 @@ int mhc_muon_step(const mhc_muon_args* a, void* stream) {
   p.steps = a->steps;
   p.eps = a->eps;
   std::copy(a->coeffs, a->coeffs + 3 * a->steps, p.coeffs);
-  p.momentum = a->momentum;
+  p.momentum = (float)a->momentum;
+  p.rest = (float)(1.0 - a->momentum);
   p.nesterov = a->nesterov;
   p.lr = a->lr;
   p.lr_dev = a->lr_device;

@@ -58,7 +58,7 @@ struct Params {
   double* part;              // [mats][segments][blocks][64]
   double* q;                 // [mats][P][P], P = 8 * NB
   double* exchange;          // [mats][2][P][P], what the clusters' CTAs pass on
-  float momentum;            // the update's coefficients; unused when only orthogonalising
+  float momentum, rest;      // the update's coefficients (rest = 1 - mu); unused when only orthogonalising
   int nesterov;
   float lr, decay, scale;
   const float* lr_dev;       // NULL, or the learning rate in device memory
@@ -165,9 +165,11 @@ __device__ __forceinline__ void store4(T* base, const Params& P, int r, int64_t 
 
 // momentum and the matrix that is orthogonalised, the same rounding in every
 // kernel that forms them: m' = mu m + (1 - mu) g, u = mu m' + (1 - mu) g or m'.
-__device__ __forceinline__ float new_momentum(float m, float g, float mu) { return fmaf(mu, m, (1.f - mu) * g); }
-__device__ __forceinline__ float update_of(float m1, float g, float mu, int nesterov) {
-  return nesterov ? fmaf(mu, m1, (1.f - mu) * g) : m1;
+__device__ __forceinline__ float new_momentum(const Params& P, float m, float g) {
+  return fmaf(P.momentum, m, P.rest * g);
+}
+__device__ __forceinline__ float update_of(const Params& P, float m1, float g) {
+  return P.nesterov ? fmaf(P.momentum, m1, P.rest * g) : m1;
 }
 
 // Accumulates block rows [R0, R1) of the lower triangle of u u^T over one
@@ -256,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(cons
         m[i].unpack(m1);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          m1[j] = new_momentum(m1[j], f[j], P.momentum);
-          f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
+          m1[j] = new_momentum(P, m1[j], f[j]);
+          f[j] = update_of(P, m1[j], f[j]);
         }
         store4<kVec>(M.mom[mat], P, r, col + c, m1, kGap);
       }
@@ -505,8 +507,8 @@ __global__ void __launch_bounds__(kFusedThreads) fused_kernel(const __grid_const
       rm.unpack(m1);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        m1[j] = new_momentum(m1[j], f[j], P.momentum);
-        f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
+        m1[j] = new_momentum(P, m1[j], f[j]);
+        f[j] = update_of(P, m1[j], f[j]);
       }
       store4<kVec>(mom, P, r, c, m1, gap);
     }
@@ -854,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
         float m1[4];
         m[k % kAhead].unpack(m1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = update_of(m1[j], f[j], P.momentum, P.nesterov);
+        for (int j = 0; j < 4; ++j) f[j] = update_of(P, m1[j], f[j]);
       }
       if (k + kAhead < kK) fetch(mat, col, k + kAhead);
 #pragma unroll

@@ -663,7 +663,7 @@ void muon_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList 
   a.nesterov = nesterov ? 1 : 0;
   a.coeffs = coeffs.data();
   a.eps = eps;
-  a.momentum = (float)momentum;
+  a.momentum = momentum;
   a.weight_decay = (float)weight_decay;
   a.scale = (float)scale;
   a.lr = (float)lr;

@@ -147,17 +147,16 @@ def test_muon_step_against_float64(L, R, C, pdt, gdt, nesterov):
     mhc_muon_step(p, g, m, lr, momentum=mu, nesterov=nesterov, weight_decay=wd, scale=scale)
     torch.cuda.synchronize()
     f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))   # noqa: E731  the coefficients as the kernels hold them
-    mu32 = f32(mu)
-    m64 = mu32 * m0.double() + (1 - mu32) * g.double()
-    mag = mu32 * m0.double().abs() + (1 - mu32) * g.double().abs()
-    _near("momentum", m, m64, 3 * U32 * mag)   # 1 - mu, its product and the fused sum, a rounding each
+    m64 = mu * m0.double() + (1 - mu) * g.double()
+    mag = mu * m0.double().abs() + (1 - mu) * g.double().abs()
+    _near("momentum", m, m64, 3 * U32 * mag)   # mu or 1 - mu, a product and the fused sum, a rounding each
     # the direction from the momentum as stored; with nesterov u carries three more roundings, which the iteration
     # (slope at most 1.1 G for these coefficients, twice for the norm) turns into an error spread over the matrix
-    u = mu32 * m.double() + (1 - mu32) * g.double() if nesterov else m.double()
+    u = mu * m.double() + (1 - mu) * g.double() if nesterov else m.double()
     want_o = O.newton_schulz(u, NEWTON_SCHULZ_COEFFS, 1e-7)
     bound = _bound(u, want_o, NEWTON_SCHULZ_COEFFS)
     if nesterov:
-        umag = (mu32 * m.double().abs() + (1 - mu32) * g.double().abs())
+        umag = (mu * m.double().abs() + (1 - mu) * g.double().abs())
         spread = 2.2 * _gain(NEWTON_SCHULZ_COEFFS) * 3 * U32 * umag.norm(dim=(-2, -1)) / u.norm(dim=(-2, -1))
         bound = bound + spread[:, None, None]
     keep, step = 1 - f32(lr) * f32(wd), f32(lr) * f32(scale)
