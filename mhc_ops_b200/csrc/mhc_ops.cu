@@ -1286,10 +1286,13 @@ OrthoPlan ortho_plan(int64_t count, int rows, int cols, int sms) {
   const int64_t least = all / p.gram_ctas;
   p.segments = (int)((p.chunks + least - 1) / least + 1);
   // Application: 32 columns to a warp at a time.  Four warps to a CTA, one on each
-  // of an SM's matrix pipes, where that spreads the columns over more SMs.
+  // of an SM's matrix pipes, where that spreads the columns over more SMs; always
+  // above 24 rows, where two such CTAs instead of one of eight warps share an SM and
+  // do not wait at the same places (1 x 80 x 32768, whole update: 93 -> 78 us).
   const int64_t width = (p.C + 31) / 32, slots = (int64_t)sms * ortho::apply_occupancy(p.NB);
-  p.apply_warps = (int64_t)p.mats * ((width + 7) / 8) < slots ? 4 : 8;
-  p.apply_ctas = (int)std::min<int64_t>((int64_t)p.mats * ((width + p.apply_warps - 1) / p.apply_warps), slots);
+  p.apply_warps = p.NB > 3 || (int64_t)p.mats * ((width + 7) / 8) < slots ? 4 : 8;
+  p.apply_ctas = (int)std::min<int64_t>((int64_t)p.mats * ((width + p.apply_warps - 1) / p.apply_warps),
+                                        p.NB > 3 ? 2 * slots : slots);
   p.q_off = align_up((size_t)p.mats * p.segments * ortho::lower_blocks(p.NB) * 64 * sizeof(double), kWsAlign);
   const size_t square = (size_t)p.mats * 64 * p.NB * p.NB * sizeof(double);
   p.exchange_off = align_up(p.q_off + square, kWsAlign);
