@@ -1355,8 +1355,41 @@ int ortho_iterate_cluster(const OrthoPlan& pl, const ortho::Params& p, cudaStrea
   return launch_behind(kernel, pl.mats * cluster, 64 * NB, smem, cluster, s, p);
 }
 
+// Whether the current device runs clusters of ten CTAs, beyond the portable
+// eight (a partition of a GPU may not).  Asked once per device, before anything
+// of a call is launched, so that no update stops half way.
+int ortho_large_clusters(bool* yes) {
+  static std::atomic<int> known[64];   // 0 not asked, 1 yes, 2 no
+  int dev = 0;
+  MHC_CUDA_TRY(cudaGetDevice(&dev));
+  int k = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (k == 0) {
+    auto kernel = ortho::iterate_cluster_kernel<10, 1>;
+    constexpr int smem = (int)ortho::cluster_smem<10, 1>();
+    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(10);
+    cfg.blockDim = dim3(640);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 10;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const bool ok = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+    if (!ok) (void)cudaGetLastError();
+    k = ok ? 1 : 2;
+    if (dev < 64) known[dev].store(k, std::memory_order_relaxed);
+  }
+  *yes = k == 1;
+  return MHC_OK;
+}
+
 template <int NB>
-int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, cudaStream_t s) {
+int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, [[maybe_unused]] bool clusters, cudaStream_t s) {
   if constexpr (NB <= ortho::kSmallBlocks) {
     auto kernel = ortho::iterate_small_kernel<NB>;
     constexpr int smem = (int)ortho::small_smem<NB>();
@@ -1364,8 +1397,9 @@ int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, cudaStre
     return launch_behind(kernel, pl.mats, 32 * ortho::small_warps(NB), smem, 1, s, p);
   } else {
     // a row block to a CTA while the device holds all the clusters at once, else two
-    if constexpr (NB % 2 == 0)
-      if (pl.mats * NB > sms) return ortho_iterate_cluster<NB, 2>(pl, p, s);
+    if constexpr (NB % 2 == 0) {
+      if (pl.mats * NB > sms || !clusters) return ortho_iterate_cluster<NB, 2>(pl, p, s);
+    }
     return ortho_iterate_cluster<NB, 1>(pl, p, s);
   }
 }
@@ -1391,9 +1425,12 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
   if (gs > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
   if (as > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
   int st;
+  bool clusters = true;
+  if constexpr (NB > 8)
+    if ((st = ortho_large_clusters(&clusters))) return st;
   gram<<<pl.gram_ctas, ortho::kThreads, gs, s>>>(p, m);
   if ((st = after_launch())) return st;
-  if ((st = ortho_iterate<NB>(pl, p, sms, s))) return st;
+  if ((st = ortho_iterate<NB>(pl, p, sms, clusters, s))) return st;
   return launch_behind(apply, pl.apply_ctas, 32 * pl.apply_warps, as, 1, s, p, m);
 }
 

@@ -61,7 +61,7 @@ def _near(name, got, want, bound):
 # chunk, odd widths, more rows than columns, several launches' worth of partial sums
 SHAPES = [(1, 3, 16), (1, 8, 1024), (2, 15, 100), (1, 24, 16384), (3, 24, 131), (1, 35, 10005), (2, 48, 640),
           (1, 63, 448), (2, 80, 2048), (1, 80, 81), (1, 1, 1), (1, 1, 5000), (1, 5, 1), (2, 80, 7), (1, 4096, 24),
-          (1, 300, 80), (1, 17, 17), (1, 40, 4096), (1, 64, 4100), (1, 9, 33000)]
+          (1, 300, 80), (20, 80, 130), (26, 63, 200), (30, 48, 96), (1, 17, 17), (1, 40, 4096), (1, 64, 4100), (1, 9, 33000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -184,8 +184,10 @@ def test_lists_lr_tensor_decay_alone_and_unlisted_neighbours():
     assert ((q - q0 * 0.95).abs() <= 3 * U32 * q0.abs()).all()
 
 
-def test_determinism_and_captured_schedule():
-    p, g, m = _muon_inputs(3, 24, 2048, 31, torch.float32, torch.float32)
+# one launch, a CTA a matrix, a cluster a matrix (ten CTAs, and five when there are many matrices)
+@pytest.mark.parametrize("L,R,C", [(3, 24, 512), (3, 24, 2048), (2, 80, 1024), (20, 80, 260)])
+def test_determinism_and_captured_schedule(L, R, C):
+    p, g, m = _muon_inputs(L, R, C, 31, torch.float32, torch.float32)
     sp, sm, lr = p.clone(), m.clone(), torch.full((1,), 0.1, device="cuda")
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
