@@ -1156,8 +1156,10 @@ struct RopePlan {
   size_t smem;
 };
 
-// CTAs of the persistent kernels at most, so also rows of the backward's weight-gradient partials.
+// CTAs of the persistent vector kernels at most, and of the other backward: rows
+// of weight-gradient partials.
 int rope_max_blocks(int sms) { return sms * 2; }
+int rope_max_rows(int sms) { return sms * 4; }
 
 RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, int sms) {
   RopePlan r{};
@@ -1200,7 +1202,7 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   }
   const int64_t tok_per_cta = rope::kWarps / p.parts;
   const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
-  r.blocks = (int)std::min<int64_t>(want, r.vec || backward ? rope_max_blocks(sms) : (int64_t)sms * 16);
+  r.blocks = (int)std::min<int64_t>(want, r.vec ? rope_max_blocks(sms) : backward ? rope_max_rows(sms) : sms * 16);
   r.smem = (size_t)rope::kWarps * sizeof(float) * (p.rot + (backward ? 2 * p.d : 0));   // the other kernels'
   return r;
 }
@@ -1222,24 +1224,27 @@ int rope_launch_vec(const rope::Params& p, const RopePlan& r, bool backward, cud
   return after_launch();
 }
 
+template <class T, bool kInter, int kP>
+int rope_launch_any(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
+  auto kernel = backward ? rope::bwd_any_kernel<T, kInter, kP> : rope::fwd_any_kernel<T, kInter, kP>;
+  if (r.smem > 48 * 1024)
+    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.smem));
+  kernel<<<r.blocks, rope::kThreads, r.smem, s>>>(p);
+  return after_launch();
+}
+
 template <class T, bool kInter>
 int rope_launch(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
-  if (r.vec) {
-    switch (r.gshift) {
-      case 2: return rope_launch_vec<T, kInter, 2>(p, r, backward, s);
-      case 3: return rope_launch_vec<T, kInter, 3>(p, r, backward, s);
-      case 4: return rope_launch_vec<T, kInter, 4>(p, r, backward, s);
-      default: return rope_launch_vec<T, kInter, 5>(p, r, backward, s);
-    }
+  if (!r.vec)
+    return p.d <= 128   ? rope_launch_any<T, kInter, 2>(p, r, backward, s)
+           : p.d <= 256 ? rope_launch_any<T, kInter, 4>(p, r, backward, s)
+                        : rope_launch_any<T, kInter, 16>(p, r, backward, s);
+  switch (r.gshift) {
+    case 2: return rope_launch_vec<T, kInter, 2>(p, r, backward, s);
+    case 3: return rope_launch_vec<T, kInter, 3>(p, r, backward, s);
+    case 4: return rope_launch_vec<T, kInter, 4>(p, r, backward, s);
+    default: return rope_launch_vec<T, kInter, 5>(p, r, backward, s);
   }
-  if (backward) {
-    MHC_CUDA_TRY(cudaFuncSetAttribute(rope::bwd_any_kernel<T, kInter>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)(rope::kWarps * 3 * rope::kMaxD * sizeof(float))));
-    rope::bwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
-  } else {
-    rope::fwd_any_kernel<T, kInter><<<r.blocks, rope::kThreads, r.smem, s>>>(p);
-  }
-  return after_launch();
 }
 
 int rope_dispatch(const mhc_qk_args* a, const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
@@ -2062,7 +2067,7 @@ int mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t d, size_t* bytes
   if (tokens < 0 || d < 1 || d > rope::kMaxD) return MHC_ERR_BAD_SHAPE;
   int sms = 0;
   if (int st = current_sm_count(&sms)) return st;
-  *bytes = (size_t)std::min<int64_t>(std::max<int64_t>(tokens, 1), rope_max_blocks(sms)) * 2 * d * sizeof(float);
+  *bytes = (size_t)std::min<int64_t>(std::max<int64_t>(tokens, 1), rope_max_rows(sms)) * 2 * d * sizeof(float);
   return MHC_OK;
 }
 

@@ -219,6 +219,8 @@ constexpr size_t gram_smem() {
 // the next chunk's loads are in flight while the warps multiply this one, each
 // taking its share of a chunk's columns.  With momentum the kernel also forms
 // and writes the new momentum; the thread that loads an element writes it.
+// 64 x 24 x 16384 with momentum: 53 us, 302 MB at 5.7 TB/s.  8 x 80 x 32768:
+// 90 us, 0.92 G multiply-adds, 55% of the matrix pipe's rate.
 template <int NB, class T, bool kMom, bool kVec>
 __global__ void __launch_bounds__(kThreads, gram_occupancy(NB)) gram_kernel(const __grid_constant__ Params P,
                                                                            const __grid_constant__ Mats M) {
@@ -364,6 +366,7 @@ __device__ __forceinline__ double inverse_norm(const double* A, int rows, int st
 // the lower triangle (products of commuting symmetric matrices are symmetric;
 // Y's rows serve as its columns) and another for the second product of a step.
 // What is left is latency: 13 dependent products of at most 10 instructions.
+// Five steps: 3.9 us for 8 rows, 7 for 24, 12 for 35.
 constexpr int kSmallBlocks = 5;
 constexpr int small_warps(int NB) { return 2 * lower_blocks(NB); }
 template <int NB>
@@ -466,6 +469,7 @@ __global__ void __launch_bounds__(32 * small_warps(NB)) iterate_small_kernel(con
 // memory between the Gram product, the iteration and the application.  One CTA's
 // matrix pipe takes about 4 cycles a product, so the limit is 3,000 of them,
 // some 6 us, about what three kernels cost in launches and starts alone.
+// 8 x 1024: 7 us against 10 in three kernels, and 10 a call against 15.
 constexpr int kFusedBlocks = 3;
 constexpr int kFusedThreads = 384;   // 12 warps: 24 rows' iteration needs as many
 constexpr int kFusedWarps = kFusedThreads / 32;
@@ -587,7 +591,7 @@ __global__ void __launch_bounds__(kFusedThreads) fused_kernel(const __grid_const
 // (the L2): a CTA's stores into the others' shared memory took 320 cycles for
 // each of them, 3,200 a step at ten CTAs.  Two warps have a block column,
 // one for each chain of products; every lane keeps its two elements of a strip
-// in registers.
+// in registers.  Five steps on 80 rows: 22 us, about 4 of them a step.
 template <int NB, int kSP>
 constexpr size_t cluster_smem() {
   return (size_t)(8 * NB + 5 * 8 * kSP) * ns_stride(NB) * sizeof(double);
@@ -742,11 +746,16 @@ __global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_c
 // products whose columns lie four apart; their results leave it eight
 // neighbouring columns 8 (l % 4) .. of rows l / 4 + 8 i.  So both ends are whole
 // vectors (element by element the columns of a product lie side by side instead,
-// for the lanes' sake) and nothing goes through shared memory but Q and the old parameters,
-// which are fetched there (cp.async, by the lane that updates them) while the
+// for the lanes' sake) and nothing goes through shared memory but Q and the old
+// parameters, which are fetched there (cp.async, by the lane that updates them) while the
 // products run.  The next columns' first rows are loaded before this step's
 // results are stored.  With few rows all of a step's loads are in registers at
 // once instead, and other warps' work covers them.
+// 64 x 24 x 16384, update: 76 us, 403 MB at 5.3 TB/s.  8 x 80 x 32768: 150 us,
+// 1.68 G multiply-adds, 61% of the matrix pipe's rate; taking out the stores, the
+// parameters or the loads gains 10 us each, so no single one of them holds it.
+// Turns at the pipe for the two warps that share one (288 us a call instead of
+// 274) and 16 warps of half the rows each (283) were slower.
 constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
 // row loads in flight; element by element they are all that hides their latency
 constexpr int apply_ahead(int NB, bool vec) { return NB <= 3 || (!vec && NB == 5) ? 2 * NB : !vec && NB == 6 ? 6 : 4; }

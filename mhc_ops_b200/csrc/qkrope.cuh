@@ -337,6 +337,9 @@ __device__ __forceinline__ bool lane_unit(const Params& P, int lane, int& u, int
 
 // Forward.  The side's weights are folded into the turn's coefficients once per
 // token and side, so that a pair costs three packed instructions each way.
+// Memory bounds it: 72 us at B=4, S=4096, 32+8+8 heads of 128, bf16, 403 MB at
+// 5.6 TB/s (a copy of the same rows: 65 us).  A few tokens are bound by the
+// launch: 4.7 us for one.
 template <class T, bool kInter, int kGS>
 __global__ void __launch_bounds__(kThreads, 2) fwd_vec_kernel(const __grid_constant__ Params P) {
   __shared__ __align__(16) float sw[2][512];
@@ -449,7 +452,9 @@ __global__ void __launch_bounds__(kThreads, 2) fwd_vec_kernel(const __grid_const
 // Backward.  Each lane keeps the weight gradients of its 16 elements: in
 // registers over a side's head groups, in its own shared-memory slots over
 // tokens.  The CTA's warps are added in warp order and the CTA's row written for
-// the finalize kernel, so repeated calls give the same bits.
+// the finalize kernel, so repeated calls give the same bits.  113 us for the
+// forward's tokens, 604 MB at 5.3 TB/s; its sums, angles and weights fill 128
+// registers, and of 16 warps an SM 57% of the issue slots are used.
 template <class T, bool kInter, int kGS>
 __global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const __grid_constant__ Params P) {
   __shared__ __align__(16) float sw[2][512];
@@ -642,16 +647,31 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const __grid_const
   }
 }
 
-// Any head width, stride and alignment: a warp per head row, lane l the pairs
-// l, l + 32, ... and the passing elements likewise.  Dynamic shared memory per
-// warp: the token's cos and sin [rot/2] and, in the backward, the weight
-// gradients [2][d] of the warp (a lane only ever touches its own columns).
+// ------------------------------------------------------------ any width, stride, alignment
+// A warp per head row, lane l the pairs l, l + 32, ..: the rotated ones, then
+// the passing elements two by two (the last of an odd number alone).  A row is
+// read once, into registers, kP pairs a lane (2 up to d = 128, 4 up to 256, else 16).
+// Dynamic shared memory per warp: the token's cos and sin [rot/2] and, in the
+// backward, the weight gradients [2][d] of the warp (a lane only ever touches its
+// own columns).
+template <bool kInter>
+__device__ __forceinline__ bool pair_places(const Params& P, int p, int& ia, int& ib) {
+  const int half = P.rot / 2;
+  if (p < half) {
+    ia = kInter ? 2 * p : p;
+    ib = kInter ? 2 * p + 1 : p + half;
+    return true;
+  }
+  ia = 2 * p;   // rot + 2 (p - half)
+  ib = 2 * p + 1;
+  return false;
+}
 __device__ __forceinline__ void head_side(const Params& P, int h, int& side, int& hh) {
   side = h < P.heads[0] ? 0 : h < P.heads[0] + P.heads[1] ? 1 : 2;
   hh = h - (side > 0 ? P.heads[0] : 0) - (side > 1 ? P.heads[1] : 0);
 }
 
-template <class T, bool kInter>
+template <class T, bool kInter, int kP>
 __global__ void __launch_bounds__(kThreads) fwd_any_kernel(const __grid_constant__ Params P) {
   extern __shared__ float dyn[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -673,32 +693,45 @@ __global__ void __launch_bounds__(kThreads) fwd_any_kernel(const __grid_constant
       head_side(P, h, side, hh);
       const T* x = row<T>(P.x[side], b, s, hh);
       T* y = const_cast<T*>(row<T>(P.out[side], b, s, hh));
-      if (side == 2) {
-        for (int i = lane; i < P.d; i += 32) store1(y + i, load1(x + i) * sc);
-        continue;
+      const float* w = side < 2 ? P.w[side] : nullptr;
+      float xa[kP], xb[kP], sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        int ia, ib;
+        pair_places<kInter>(P, lane + 32 * i, ia, ib);
+        xa[i] = ia < P.d ? load1(x + ia) * sc : 0.f;
+        xb[i] = ib < P.d ? load1(x + ib) * sc : 0.f;
       }
-      float sq = 0.f;
-      for (int i = lane; i < P.d; i += 32) {
-        const float z = load1(x + i) * sc;
-        sq = fmaf(z, z, sq);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        sq = fmaf(xa[i], xa[i], sq);
+        sq = fmaf(xb[i], xb[i], sq);
       }
-      sq = warp_sum(sq);
-      const float r = rsqrtf(fmaf(sq, inv_d, P.eps));
-      const float* w = P.w[side];
-      for (int i = lane; i < half; i += 32) {
-        const int ia = kInter ? 2 * i : i, ib = kInter ? 2 * i + 1 : i + half;
-        const float a = load1(x + ia) * sc * r * (w ? MHC_LDG(w + ia) : 1.f);
-        const float c = load1(x + ib) * sc * r * (w ? MHC_LDG(w + ib) : 1.f);
-        store1(y + ia, a * cs[i] - c * sn[i]);
-        store1(y + ib, a * sn[i] + c * cs[i]);
+      const float r = side == 2 ? 1.f : rsqrtf(fmaf(warp_sum(sq), inv_d, P.eps));
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        int ia, ib;
+        const bool turned = pair_places<kInter>(P, lane + 32 * i, ia, ib) && side != 2;
+        if (ia < P.d) {
+          float a = xa[i] * r, c = xb[i] * r;
+          if (w) {
+            a *= MHC_LDG(w + ia);
+            if (ib < P.d) c *= MHC_LDG(w + ib);
+          }
+          if (turned) {
+            const float cc = cs[lane + 32 * i], ss = sn[lane + 32 * i], a0 = a;
+            a = a0 * cc - c * ss;
+            c = a0 * ss + c * cc;
+          }
+          store1(y + ia, a);
+          if (ib < P.d) store1(y + ib, c);
+        }
       }
-      for (int i = P.rot + lane; i < P.d; i += 32)
-        store1(y + i, load1(x + i) * sc * r * (w ? MHC_LDG(w + i) : 1.f));
     }
   }
 }
 
-template <class T, bool kInter>
+template <class T, bool kInter, int kP>
 __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const __grid_constant__ Params P) {
   extern __shared__ float dyn[];
   __shared__ float sds[kWarps];
@@ -727,56 +760,64 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const __grid_constant
         const T* x = row<T>(P.x[side], b, s, hh);
         const T* dy = row<T>(P.dy[side], b, s, hh);
         T* dx = const_cast<T*>(row<T>(P.out[side], b, s, hh));
-        if (side == 2) {
-          for (int i = lane; i < P.d; i += 32) {
-            const float g = load1(dy + i);
-            ds = fmaf(load1(x + i), g, ds);
-            store1(dx + i, g * sc);
-          }
-          continue;
+        const float* w = side < 2 ? P.w[side] : nullptr;
+        float xa[kP], xb[kP], ga[kP], gb[kP];   // x; da = Rot^T dy
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+          int ia, ib;
+          pair_places<kInter>(P, lane + 32 * i, ia, ib);
+          xa[i] = ia < P.d ? load1(x + ia) : 0.f;
+          xb[i] = ib < P.d ? load1(x + ib) : 0.f;
+          ga[i] = ia < P.d ? load1(dy + ia) : 0.f;
+          gb[i] = ib < P.d ? load1(dy + ib) : 0.f;
         }
-        const float* w = P.w[side];
-        float* g = gw + side * P.d;
         float sq = 0.f, dot = 0.f;
-        for (int i = lane; i < P.d; i += 32) {
-          const float z = load1(x + i) * sc;
-          sq = fmaf(z, z, sq);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+          int ia, ib;
+          const bool turned = pair_places<kInter>(P, lane + 32 * i, ia, ib) && side != 2;
+          if (turned) {
+            const float cc = cs[lane + 32 * i], ss = sn[lane + 32 * i], g0 = ga[i];
+            ga[i] = g0 * cc + gb[i] * ss;
+            gb[i] = gb[i] * cc - g0 * ss;
+          }
+          const float za = xa[i] * sc, zb = xb[i] * sc;
+          sq = fmaf(za, za, sq);
+          sq = fmaf(zb, zb, sq);
+          dot = fmaf(w && ia < P.d ? ga[i] * MHC_LDG(w + ia) : ga[i], xa[i], dot);
+          dot = fmaf(w && ib < P.d ? gb[i] * MHC_LDG(w + ib) : gb[i], xb[i], dot);
         }
-        // da of a pair, dn = w da
-        for (int i = lane; i < half; i += 32) {
-          const int ia = kInter ? 2 * i : i, ib = kInter ? 2 * i + 1 : i + half;
-          const float ya = load1(dy + ia), yb = load1(dy + ib);
-          const float da = ya * cs[i] + yb * sn[i], db = yb * cs[i] - ya * sn[i];
-          dot = fmaf(da * (w ? MHC_LDG(w + ia) : 1.f), load1(x + ia), dot);
-          dot = fmaf(db * (w ? MHC_LDG(w + ib) : 1.f), load1(x + ib), dot);
+        dot = warp_sum(dot);   // sum(dn x); sum(v dv_out) on value rows
+        float sr = sc, m = 0.f;
+        if (side == 2) {
+          if (lane == 0) ds += dot;
+        } else {
+          const float r = rsqrtf(fmaf(warp_sum(sq), inv_d, P.eps));
+          sr = sc * r;
+          m = sr * dot * inv_d;
+          if (lane == 0) ds += P.eps * r * r * r * dot;
         }
-        for (int i = P.rot + lane; i < P.d; i += 32)
-          dot = fmaf(load1(dy + i) * (w ? MHC_LDG(w + i) : 1.f), load1(x + i), dot);
-        sq = warp_sum(sq);
-        dot = warp_sum(dot);
-        const float r = rsqrtf(fmaf(sq, inv_d, P.eps));
-        const float sr = sc * r;
-        const float m = sr * dot * inv_d;
-        if (lane == 0) ds += P.eps * r * r * r * dot;
-        for (int i = lane; i < half; i += 32) {
-          const int ia = kInter ? 2 * i : i, ib = kInter ? 2 * i + 1 : i + half;
-          const float ya = load1(dy + ia), yb = load1(dy + ib);
-          const float da = ya * cs[i] + yb * sn[i], db = yb * cs[i] - ya * sn[i];
-          const float na = load1(x + ia) * sr, nb = load1(x + ib) * sr;
-          g[ia] = fmaf(na, da, g[ia]);
-          g[ib] = fmaf(nb, db, g[ib]);
-          store1(dx + ia, sr * (da * (w ? MHC_LDG(w + ia) : 1.f) - na * m));
-          store1(dx + ib, sr * (db * (w ? MHC_LDG(w + ib) : 1.f) - nb * m));
-        }
-        for (int i = P.rot + lane; i < P.d; i += 32) {
-          const float da = load1(dy + i), n = load1(x + i) * sr;
-          g[i] = fmaf(n, da, g[i]);
-          store1(dx + i, sr * (da * (w ? MHC_LDG(w + i) : 1.f) - n * m));
+        float* g = gw + (side == 0 ? 0 : P.d);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
+          int ia, ib;
+          pair_places<kInter>(P, lane + 32 * i, ia, ib);
+          if (ia < P.d) {
+            const float na = xa[i] * sr;
+            if (side != 2) g[ia] = fmaf(na, ga[i], g[ia]);
+            const float dn = w ? ga[i] * MHC_LDG(w + ia) : ga[i];
+            store1(dx + ia, sr * (side == 2 ? dn : dn - na * m));
+          }
+          if (ib < P.d) {
+            const float nb = xb[i] * sr;
+            if (side != 2) g[ib] = fmaf(nb, gb[i], g[ib]);
+            const float dn = w ? gb[i] * MHC_LDG(w + ib) : gb[i];
+            store1(dx + ib, sr * (side == 2 ? dn : dn - nb * m));
+          }
         }
       }
     }
     if (P.d_row_scale) {
-      ds = warp_sum(ds);
       if (lane == 0) sds[warp] = ds;
       __syncthreads();
       if (part == 0 && lane == 0 && t < P.T) {
