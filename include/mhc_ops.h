@@ -44,7 +44,7 @@ extern "C" {
 typedef enum mhc_status {
   MHC_OK = 0,
   MHC_ERR_NULL_POINTER = 1,        /* a required pointer is NULL */
-  MHC_ERR_BAD_SHAPE = 2,           /* T < 0, n outside [1,8], D < 1, or overflow */
+  MHC_ERR_BAD_SHAPE = 2,           /* T < 0, n outside [1,8], D < 1, overflow; of the other entry points a size or option outside theirs */
   MHC_ERR_MISALIGNED = 3,          /* a pointer is not 16-byte aligned */
   MHC_ERR_WORKSPACE_TOO_SMALL = 4, /* workspace_bytes below the *_workspace_size answer */
   MHC_ERR_CUDA = 5,                /* a CUDA runtime/driver call failed (see mhc_last_cuda_error) */
@@ -394,9 +394,11 @@ MHC_API int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* args, void* stream);
  * major; min(rows, cols) <= 80, the n*n + 2n rows of phi for n <= 8):
  *   X = U / (|U|_F + eps), then per step X <- a X + (b A + c A^2) X, A = X X^T.
  * coeffs holds `steps` (1 to 16) triples a, b, c on the host.  The matrices'
- * pointers are host arrays.  eps >= 1e-20.  The small iteration runs in 64
- * bits, the application in 32; results do not depend on `count`.  The
- * workspace need not be zeroed.  No counterpart in the reference. */
+ * pointers are host arrays.  eps >= 1e-20.  All sums run in 64 bits and the
+ * result is rounded once.  Every matrix is treated alone; only the order of the
+ * 64-bit sums goes by count, rows and cols (and the device), so repeated calls
+ * return identical bytes.  The workspace need not be zeroed.  No counterpart in
+ * the reference. */
 typedef struct mhc_ortho_args {
   const void* const* in;
   void* const* out;            /* may be `in` */

@@ -13,8 +13,9 @@ layer in one call::
     phi <- (1 - lr weight_decay) phi - lr scale orthogonalised(u)
 
 The shorter side of a matrix may have up to 80 rows, the ``n*n + 2n`` rows of
-phi at n = 8.  Sums over the long side and the iteration run in 64 bits, the
-last product in 32.  The reference has no optimiser.
+phi at n = 8.  All sums run in 64 bits (32 would lose small singular values,
+which the steps lift a few hundred times) and the result is rounded once.  The
+reference has no optimiser.
 """
 from __future__ import annotations
 
@@ -52,7 +53,7 @@ def mhc_orthogonalize(g, coeffs=NEWTON_SCHULZ_COEFFS, eps: float = 1e-7):
     equal matrices, fp32 or bf16, with ``min(rows, cols) <= 80``.
 
     Returns the same kind (a list for a sequence) in the input's type.  Every
-    matrix is treated alone: the result does not depend on its neighbours.
+    matrix is treated alone; repeated calls return the same bits.
     """
     out = ops.orthogonalize(_list(g, "g"), _coeffs(coeffs), eps)
     return out[0] if torch.is_tensor(g) else out

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from mhc_ops_b200 import (NEWTON_SCHULZ_COEFFS, mhc_backward_manual, mhc_forward_pre, mhc_forward_pre_fused_norm,
-                          mhc_muon_step, mhc_post_fn, mhc_pre, mhc_qk_norm_rope, mhc_qkv_norm_rope_fn)
+                          mhc_muon_step, mhc_orthogonalize, mhc_post_fn, mhc_pre, mhc_qk_norm_rope,
+                          mhc_qk_norm_rope_backward, mhc_qkv_norm_rope_fn)
 from mhc_ops_b200.backward import param_grad_numel
 from mhc_ops_b200.dist import DataParallelMHC
 from mhc_ops_b200.synthetic import make_inputs
@@ -110,6 +111,71 @@ def test_row_factor_stands_in_for_the_norm_before_the_projection():
     for a, b in zip(got, want):
         err = (a.double() - b).norm(dim=-1) / b.norm(dim=-1)
         assert err.max() <= 3 * 2.0 ** -8, float(err.max())
+
+
+def test_row_factor_carries_its_gradient_to_h_in():
+    """h_in's gradient through projection and row factor, dqkv w - drow_scale rstd^3 h_in / D, against float64 autograd.
+
+    dqkv is right to (d/32 + 40) 2^-24 of its terms (tests/test_qkrope_gpu.py), the projection's sums of 512
+    products add as much again as they have terms, at worst 512 2^-24 of the sum of magnitudes; the norms of the two
+    sums differ from sqrt by less than 10: 1e-3 of the gradient's norm bounds all of it, and the row factor's part
+    (eps is large here, so that it is not lost below that) is a tenth of the whole or more."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")   # noqa: E731
+    eps, f = 0.3, (10000.0 ** (-torch.arange(d // 2, device="cuda") / (d // 2))).float()
+    h, w = rnd(B, S, D), rnd((HQ + 2 * HK) * d, D) / D ** 0.5
+    up = rnd(B, S, HQ + 2 * HK, d)
+    rstd = 1.0 / torch.sqrt((h * h).mean(-1) + 1e-6)
+    qkv = (h @ w.T).view(B, S, -1, d)
+    parts = (HQ, HK, HK)
+    q, k, v = qkv.split(parts, dim=2)
+    dq, dk, dv = up.split(parts, dim=2)
+    dqkv = torch.empty_like(qkv)
+    out = mhc_qk_norm_rope_backward(q, k, None, f, dq, dk, v=v, dv_out=dv, row_scale=rstd, eps=eps,
+                                    grad_out=dqkv.split(parts, dim=2))
+    through = -out[5][..., None] * rstd[..., None] ** 3 * h / D
+    got = dqkv.flatten(2) @ w + through
+    x = h.double().requires_grad_()
+    y = (x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6)) @ w.double().T
+    y = y.view(B, S, -1, d)
+    angle = O.angles(None, f, B, S)
+    o = [O.norm_rope(y[:, :, :HQ], None, None, angle, eps, False),
+         O.norm_rope(y[:, :, HQ:HQ + HK], None, None, angle, eps, False), y[:, :, HQ + HK:]]
+    want, = torch.autograd.grad(torch.cat(o, dim=2), x, up.double())
+    assert (got - want).norm() <= 1e-3 * want.norm()
+    assert through.norm() >= 0.1 * want.norm() or (got - through - want).norm() >= 5e-3 * want.norm()
+
+
+def test_calls_from_two_threads_on_two_streams():
+    """Calls that overlap share nothing: each thread's results equal the same calls made alone."""
+    import threading
+    u = [torch.randn(4, 24, 3000, device="cuda"), torch.randn(3, 80, 700, device="cuda")]
+    q = [torch.randn(2, 300, 4, 64, device="cuda").bfloat16() for _ in range(2)]
+    f = torch.rand(32, device="cuda")
+
+    def work(i):
+        return (mhc_orthogonalize(u[i]),) + mhc_qk_norm_rope_backward(q[i], q[i], None, f, q[i], q[i], torch.ones(
+            64, device="cuda"))[:4]
+
+    alone = [work(0), work(1)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[i] = work(i)
+        s.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        for a, b in zip(got[i], alone[i]):
+            assert a is None and b is None or torch.equal(a, b)
 
 
 def test_data_parallel_object_updates_phi():
