@@ -330,7 +330,7 @@ MHC_API int mhc_post_bwd(const mhc_post_bwd_args* args, void* stream);
  * (src/forward/golden.py:62-63).
  * Tensors are [batch, seq, heads, d] of `dtype` with unit stride along d and
  * the given strides in elements; positions [batch, seq] are int32 or int64
- * (position_bytes 4 or 8) or NULL, then 0 .. seq - 1.  Angles are exact to 32
+ * (position_bytes 4 or 8) or NULL, then 0 .. seq - 1.  Angles are right to 32
  * bits for |position| < 2^31.  1 <= d <= 1024, rot even and <= d; sums are 32
  * bits wide.  No workspace in the forward; inputs and outputs do not overlap.
  * 16-byte aligned tensors and strides with d and rot multiples of 16 and

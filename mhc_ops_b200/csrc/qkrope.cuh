@@ -15,9 +15,10 @@
 // (sum(x . dz), the direct form of ds, cancels down to the eps term; the line
 // above is what is left, without a division by s.)
 //
-// The angle is p f / 2pi in 64 bits, reduced to half a turn there, then one
-// sincospi in 32 bits: exact to 32 bits at any position below 2^31, without a
-// table that would have to be as long as the longest sequence.
+// The angle is p f / 2pi in 64 bits with what its products round off carried
+// along, reduced to half a turn there, then one sincospi in 32 bits turned on by
+// what rounding the angle lost: right to 32 bits at any position below 2^31,
+// without a table that would have to be as long as the longest sequence.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -140,11 +141,21 @@ __device__ __forceinline__ int64_t position(const Params& P, int b, int s) {
   return MHC_LDG(reinterpret_cast<const int*>(P.pos) + i);
 }
 
-// cos and sin of pos * f; see the head of this file.
+// cos and sin of pos * f; see the head of this file.  Without the products' low
+// parts the angle is off by up to 8 * 2^-24 at positions near 2^31; without the
+// last step by up to 1.6 * 2^-24 at any, where cos and sin round by 2^-25.
 __device__ __forceinline__ void turn(int64_t pos, float f, float& c, float& s) {
-  double rev = (double)pos * ((double)f * 0.15915494309189533577);
-  rev -= rint(rev);
-  sincospif(2.0f * (float)rev, &s, &c);
+  constexpr double kHi = 0x1.45f306dc9c883p-3, kLo = -0x1.6b01ec5417056p-57;   // 1 / 2pi
+  // products rounded by themselves: contracted into a sum, h's low part would count twice
+  const double p = __dmul_rn((double)pos, (double)f), e = fma((double)pos, (double)f, -p);
+  const double h = __dmul_rn(p, kHi);
+  const double rev = (h - rint(h)) + fma(e, kHi, fma(p, kLo, fma(p, kHi, -h)));
+  const float r = 2.0f * (float)rev;
+  const float rest = (float)(2.0 * rev - (double)r) * 3.14159265358979f;
+  sincospif(r, &s, &c);
+  const float s0 = s;
+  s = fmaf(c, rest, s);
+  c = fmaf(-s0, rest, c);
 }
 
 // The two 8-element chunks of unit u of a head row (d / 16 units).  Half-split

@@ -3,6 +3,9 @@ the per-head norms of queries and keys with the rotary rotation, and the orthogo
 Test infrastructure; torch in float64, written from the formulas alone."""
 from __future__ import annotations
 
+from decimal import Decimal, getcontext
+from fractions import Fraction
+
 import torch
 
 
@@ -63,3 +66,29 @@ def muon_step(p, g, m, lr, mu, nesterov, decay, scale, coeffs, eps):
     m = mu * m + (1 - mu) * g
     u = mu * m + (1 - mu) * g if nesterov else m
     return (1 - lr * decay) * p - lr * scale * newton_schulz(u, coeffs, eps), m
+
+
+def _inverse_two_pi():
+    """1 / (2 pi) to 60 digits, pi = 16 arctan(1/5) - 4 arctan(1/239)."""
+    getcontext().prec = 70
+
+    def arctan(n):
+        term = total = Decimal(1) / n
+        k = 1
+        while abs(term) > Decimal(10) ** -66:
+            term, k = -term / (n * n), k + 2
+            total += term / k
+        return total
+
+    return Fraction(1 / (8 * (4 * arctan(5) - arctan(239))))
+
+
+def far_angles(positions, inv_freq):
+    """position * inv_freq [len(positions), len(inv_freq)], reduced to [-pi, pi] in exact arithmetic: the angles of
+    positions at which a float64 product has lost what float32 needs."""
+    inv = _inverse_two_pi()
+    rows = []
+    for f in inv_freq.tolist():
+        g = Fraction(f) * inv
+        rows.append([float(t - round(t)) for t in (g * int(p) for p in positions.tolist())])
+    return torch.tensor(rows, dtype=torch.float64).T * (2 * torch.pi)
