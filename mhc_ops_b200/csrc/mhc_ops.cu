@@ -1161,6 +1161,11 @@ struct RopePlan {
 int rope_max_blocks(int sms) { return sms * 2; }
 int rope_max_rows(int sms) { return sms * 4; }
 
+// Dynamic shared memory of the kernels of any width.
+constexpr size_t rope_any_smem(int d, int rot, bool backward) {
+  return (size_t)rope::kWarps * sizeof(float) * (rot + (backward ? 2 * d : 0));
+}
+
 RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, int sms) {
   RopePlan r{};
   p.x[0] = rope_view(a->q);
@@ -1203,7 +1208,7 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   const int64_t tok_per_cta = rope::kWarps / p.parts;
   const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
   r.blocks = (int)std::min<int64_t>(want, r.vec ? rope_max_blocks(sms) : backward ? rope_max_rows(sms) : sms * 16);
-  r.smem = (size_t)rope::kWarps * sizeof(float) * (p.rot + (backward ? 2 * p.d : 0));   // the other kernels'
+  r.smem = rope_any_smem(p.d, p.rot, backward);
   return r;
 }
 
@@ -1227,8 +1232,11 @@ int rope_launch_vec(const rope::Params& p, const RopePlan& r, bool backward, cud
 template <class T, bool kInter, int kP>
 int rope_launch_any(const rope::Params& p, const RopePlan& r, bool backward, cudaStream_t s) {
   auto kernel = backward ? rope::bwd_any_kernel<T, kInter, kP> : rope::fwd_any_kernel<T, kInter, kP>;
-  if (r.smem > 48 * 1024)
-    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.smem));
+  // The widest head's, whatever this call's: a limit that went by the call would
+  // be lowered under another thread's launch.  Static arrays count too, so a call
+  // of just the default limit needs it raised as well; 256 wide stay far below it.
+  if constexpr (kP > 4)
+    if (int st = set_smem_limit_once(kernel, (int)rope_any_smem(rope::kMaxD, rope::kMaxD, backward))) return st;
   kernel<<<r.blocks, rope::kThreads, r.smem, s>>>(p);
   return after_launch();
 }
