@@ -1424,8 +1424,8 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
     if (pl.fused) {
       auto fused = vec ? ortho::fused_kernel<NB, T, TO, kMom, true> : ortho::fused_kernel<NB, T, TO, kMom, false>;
       const int smem = (int)ortho::fused_smem<NB>(pl.C);
-      if (smem > kDefaultSmem)
-        MHC_CUDA_TRY(cudaFuncSetAttribute(fused, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      // the largest matrix's: a limit that went by C would be lowered under another thread's launch
+      if (int st = set_smem_limit_once(fused, (int)(ortho::fused_fixed_smem<NB>() + ortho::kFusedMatrix))) return st;
       fused<<<pl.mats, ortho::kFusedThreads, smem, s>>>(p, m);
       return after_launch();
     }

@@ -474,14 +474,18 @@ constexpr int kFusedBlocks = 3;
 constexpr int kFusedThreads = 384;   // 12 warps: 24 rows' iteration needs as many
 constexpr int kFusedWarps = kFusedThreads / 32;
 __host__ __device__ constexpr int fused_stride(int C) { return (C + 31) / 32 * 32 + 4; }
+constexpr size_t kFusedMatrix = 128 * 1024;   // bytes of the matrix at most
 inline bool fused_fits(int NB, int C) {
   return NB <= kFusedBlocks && (int64_t)(lower_blocks(NB) + NB * NB) * C <= 4 * 3000 &&
-         (int64_t)8 * NB * fused_stride(C) * 4 <= 128 * 1024;
+         (int64_t)8 * NB * fused_stride(C) * 4 <= (int64_t)kFusedMatrix;
+}
+template <int NB>
+constexpr size_t fused_fixed_smem() {   // beside the matrix
+  return small_smem<NB>() + (size_t)kFusedWarps * lower_blocks(NB) * 64 * sizeof(double);
 }
 template <int NB>
 size_t fused_smem(int C) {
-  return small_smem<NB>() + (size_t)kFusedWarps * lower_blocks(NB) * 64 * sizeof(double) +
-         (size_t)8 * NB * fused_stride(C) * sizeof(float);
+  return fused_fixed_smem<NB>() + (size_t)8 * NB * fused_stride(C) * sizeof(float);
 }
 template <int NB, class T, class TO, bool kMom, bool kVec>
 __global__ void __launch_bounds__(kFusedThreads) fused_kernel(const __grid_constant__ Params P,

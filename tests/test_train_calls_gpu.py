@@ -1,11 +1,15 @@
 """Calls of the operators around a training step that the documentation allows and a single thread, a warm process
 or a plain layout never makes."""
+import ctypes
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
+
+from mhc_ops_b200 import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
@@ -30,3 +34,55 @@ for d, rot, off in ((768, 0, 0), (640, 256, 0), (704, 128, 0), (512, 512, 1)):
     res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT),
                          capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stderr[-2000:]
+
+
+def _matrix_call(C):
+    """mhc_orthogonalize of one 8 x C matrix (one launch, shared memory by C) on a stream of its own."""
+    u = torch.randn(8, C, device="cuda", generator=torch.Generator(device="cuda").manual_seed(C))
+    out, s = torch.empty_like(u), torch.cuda.Stream()
+    co = (ctypes.c_double * 3)(1.5, -0.5, 0.0)
+    src, dst = (ctypes.c_void_p * 1)(u.data_ptr()), (ctypes.c_void_p * 1)(out.data_ptr())
+    vp = lambda x: ctypes.cast(x, ctypes.c_void_p)   # noqa: E731
+    a = _lib.OrthoArgs(inp=vp(src), out=vp(dst), count=1, rows=8, cols=C, dtype=2, steps=1, coeffs=vp(co), eps=1e-7)
+    return (lambda: _lib.load().mhc_orthogonalize(ctypes.byref(a), s.cuda_stream)), out, s, (u, co, src, dst)
+
+
+def _row_call(d):
+    """mhc_qk_norm_rope_bwd of one token of d elements off the vector kernels (shared memory by d)."""
+    x = torch.randn(1, 1, 2, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d))
+    out, dk, dw, s = torch.empty_like(x), torch.empty_like(x), torch.empty(d, device="cuda"), torch.cuda.Stream()
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    heads = lambda t: _lib.Heads(t.data_ptr(), *t.stride()[:3])   # noqa: E731
+    a = _lib.QkArgs(q=heads(x), k=heads(x), batch=1, seq=1, q_heads=2, k_heads=2, d=d, rot=0, dtype=2, eps=1e-6)
+    b = _lib.QkBwdArgs(fwd=a, dq_out=heads(x), dk_out=heads(x), dq=heads(out), dk=heads(dk), dq_weight=dw.data_ptr(),
+                       workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    return (lambda: _lib.load().mhc_qk_norm_rope_bwd(ctypes.byref(b), s.cuda_stream)), out, s, (x, dk, dw, ws)
+
+
+@pytest.mark.parametrize("make,sizes", [(_matrix_call, (4000, 2000)), (_row_call, (1024, 800))])
+def test_two_threads_with_two_sizes_of_one_kernel(make, sizes):
+    """Each thread's calls all succeed: what a kernel may take of shared memory is the process's, not the call's."""
+    calls = [make(n) for n in sizes]
+    alone = []
+    for call, out, s, _ in calls:
+        s.wait_stream(torch.cuda.current_stream())
+        assert call() == 0
+        s.synchronize()
+        alone.append(out.clone())
+    torch.cuda.synchronize()
+    refused = [0, 0]
+
+    def run(i):
+        torch.cuda.set_device(0)
+        for _ in range(5000):
+            refused[i] += calls[i][0]() != 0
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert refused == [0, 0]
+    for (_, out, _, _), want in zip(calls, alone):
+        assert torch.equal(out, want)
