@@ -362,6 +362,44 @@ __device__ __forceinline__ double inverse_norm(const double* A, int rows, int st
   return 1.0 / (sqrt(tr) + eps);
 }
 
+// Block x of the lower triangle, row by row, and the first of a lane's two
+// neighbouring results in it.
+__host__ __device__ constexpr void block_place(int x, int lane, int& bi, int& bj, int& r, int& c) {
+  bi = 0;
+  while (lower_blocks(bi + 1) <= x) ++bi;
+  bj = x - lower_blocks(bi);
+  r = 8 * bi + (lane >> 2);
+  c = 8 * bj + 2 * (lane & 3);
+}
+// A result at (r, c) of the lower triangle's blocks is stored in its place and its
+// mirror image's.  In a diagonal block (r, c) and (c, r) are two lanes' results,
+// which may differ in their last bits: the one on or below the diagonal is stored,
+// in both places, so that every word has one writer and the matrix is symmetric.
+__host__ __device__ constexpr bool mirrors(int r, int c) { return r >= c; }
+__device__ __forceinline__ void put_mirrored(double* X, int stride, int r, int c, double v) {
+  if (!mirrors(r, c)) return;
+  X[r * stride + c] = v;
+  X[c * stride + r] = v;
+}
+template <int NB>
+constexpr bool one_writer_a_word() {
+  int writers[8 * NB][8 * NB] = {};
+  for (int x = 0; x < lower_blocks(NB); ++x)
+    for (int lane = 0; lane < 32; ++lane) {
+      int bi = 0, bj = 0, r = 0, c = 0;
+      block_place(x, lane, bi, bj, r, c);
+      for (int j = 0; j < 2; ++j)
+        if (mirrors(r, c + j)) {
+          ++writers[r][c + j];
+          if (r != c + j) ++writers[c + j][r];
+        }
+    }
+  for (const auto& row : writers)
+    for (int n : row)
+      if (n != 1) return false;
+  return true;
+}
+
 // The iteration on matrices of up to 40 rows, a CTA each: a warp per block of
 // the lower triangle (products of commuting symmetric matrices are symmetric;
 // Y's rows serve as its columns) and another for the second product of a step.
@@ -377,6 +415,7 @@ constexpr size_t small_smem() {
 template <int NB>
 struct SmallPlace {
   static constexpr int kB = lower_blocks(NB), S = ns_stride(NB);
+  static_assert(one_writer_a_word<NB>(), "a word of the square with no writer or with two");
   bool first, second;   // this warp has a block of the first or of the second product
   int x, r, c, fx, fy;  // its block, this lane's two results (r, c), (r, c + 1), fragment places
   __device__ __forceinline__ SmallPlace() {
@@ -384,19 +423,14 @@ struct SmallPlace {
     first = warp < kB;
     second = warp >= kB && warp < 2 * kB;
     x = second ? warp - kB : first ? warp : 0;
-    int bi = 0;
-    while (lower_blocks(bi + 1) <= x) ++bi;
-    const int bj = x - lower_blocks(bi);
-    r = 8 * bi + (lane >> 2);
-    c = 8 * bj + 2 * (lane & 3);
+    int bi, bj;
+    block_place(x, lane, bi, bj, r, c);
     fx = (8 * bi + (lane >> 2)) * S + (lane & 3);
     fy = (8 * bj + (lane >> 2)) * S + (lane & 3);
   }
-  __device__ __forceinline__ void put(double* X, double v0, double v1) const {   // a result and its mirror image
-    X[r * S + c] = v0;
-    X[r * S + c + 1] = v1;
-    X[c * S + r] = v0;
-    X[(c + 1) * S + r] = v1;
+  __device__ __forceinline__ void put(double* X, double v0, double v1) const {
+    put_mirrored(X, S, r, c, v0);
+    put_mirrored(X, S, r, c + 1, v1);
   }
 };
 // From the Gram matrix in A (all of it, behind a barrier) to Q, by a whole CTA;
@@ -457,8 +491,7 @@ __global__ void __launch_bounds__(32 * small_warps(NB)) iterate_small_kernel(con
   double v = 0.0;
 #pragma unroll 16
   for (int s = 0; s < segments; ++s) v += MHC_LD(part + (int64_t)s * (kB * 64));
-  A[pl.r * S + pl.c + odd] = v;
-  A[(pl.c + odd) * S + pl.r] = v;
+  put_mirrored(A, S, pl.r, pl.c + odd, v);
   __syncthreads();
   const double inv = iterate_small<NB>(P, pl, A, Mk, W, Q, &shared_inv);
   double* q = P.q + (int64_t)blockIdx.x * kRows * kRows;
@@ -540,11 +573,9 @@ __global__ void __launch_bounds__(kFusedThreads) fused_kernel(const __grid_const
     double v = 0.0;
 #pragma unroll
     for (int w = 0; w < kFusedWarps; ++w) v += sums[w * kB * 64 + e];
-    int bi = 0;
-    while (lower_blocks(bi + 1) <= e / 64) ++bi;
-    const int l = (e & 63) >> 1, r = 8 * bi + (l >> 2), c = 8 * (e / 64 - lower_blocks(bi)) + 2 * (l & 3) + (e & 1);
-    A[r * S + c] = v;
-    A[c * S + r] = v;
+    int bi, bj, r, c;
+    block_place(e / 64, (e & 63) >> 1, bi, bj, r, c);
+    put_mirrored(A, S, r, c + (e & 1), v);
   }
   __syncthreads();
   const SmallPlace<NB> pl;

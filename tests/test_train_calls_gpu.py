@@ -9,7 +9,7 @@ import threading
 import pytest
 import torch
 
-from mhc_ops_b200 import _lib
+from mhc_ops_b200 import _lib, mhc_orthogonalize
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
@@ -86,3 +86,21 @@ def test_two_threads_with_two_sizes_of_one_kernel(make, sizes):
     assert refused == [0, 0]
     for (_, out, _, _), want in zip(calls, alone):
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("L,R,C", [(1, 8, 1024), (1, 24, 512), (2, 24, 4096), (40, 35, 700), (3, 40, 2048)])
+def test_repeated_calls_beside_other_work_return_the_same_bytes(L, R, C):
+    """The iteration by blocks of the lower triangle, whose results and mirror images have one writer each."""
+    u = torch.randn(L, R, C, device="cuda", generator=torch.Generator(device="cuda").manual_seed(R))
+    other, x = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda")
+    want = mhc_orthogonalize(u)
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(40):
+        with torch.cuda.stream(other):
+            for _ in range(i % 4):
+                x.mul_(1.0)
+        outs.append(mhc_orthogonalize(u))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, want)
