@@ -833,26 +833,36 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
     mat = (int)(x / steps);
     col = (x - (int64_t)mat * steps) * (32 * warps) + warp * 32;
   };
-  auto fetch = [&](int mat, int64_t col, int k) {
+  auto fetch_grad = [&](int mat, int64_t col, int k) {
     const int64_t c = col + (kVec ? 4 : 1) * (lane >> 2);
     load4<kVec>(g[k % kAhead], static_cast<const T*>(M.grad[mat]), P, 4 * k + (lane & 3), c, kGap);
+  };
+  auto fetch_mom = [&](int mat, int64_t col, int k) {
+    const int64_t c = col + (kVec ? 4 : 1) * (lane >> 2);
     if (kMom) load4<kVec>(m[k % kAhead], static_cast<const float*>(M.mom[mat]), P, 4 * k + (lane & 3), c, kGap);
+  };
+  // The first rows of a step.  Momenta were written by this call's Gram kernel, so
+  // the first read of them is behind the wait: that kernel had ended when this one
+  // could start, but what it wrote is promised to be seen only from there on.
+  // Gradients, parameters and the learning rate are older than the call.
+  auto fetch_first = [&](int mat, int64_t col, bool wait) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch_grad(mat, col, k);
+    if (kMom && wait) cudaGridDependencySynchronize();
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch_mom(mat, col, k);
   };
   int loaded = -1, mat;
   int64_t col;
   // from the end: what the Gram pass touched last is the likeliest to be in the L2
   place(x1 - 1, mat, col);
-  if (kStage && x0 < x1)
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
+  if (kStage && x0 < x1) fetch_first(mat, col, true);
   for (int64_t x = x1 - 1; x >= x0; --x) {
     place(x, mat, col);
     TO* out = static_cast<TO*>(M.out[mat]);
     // this lane's eight columns of the result: half j at oc + kHalf * j, kGap apart
     const int64_t oc = col + (kVec ? 8 : 2) * (lane & 3);
-    if constexpr (!kStage)
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) fetch(mat, col, k);
+    if constexpr (!kStage) fetch_first(mat, col, loaded < 0);
     if constexpr (kStage) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
@@ -877,9 +887,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     if (mat != loaded) {   // the same for the whole CTA
-      // gradients and momenta were ready when this kernel could start; Q is
-      // not before the iteration has ended
-      cudaGridDependencySynchronize();
+      cudaGridDependencySynchronize();   // Q is ready when the iteration has ended
       __syncthreads();
       const double* q = P.q + (int64_t)mat * kRows * kRows;
       for (int e = threadIdx.x; e < kRows * kRows; e += blockDim.x) Q[e / kRows * S + e % kRows] = MHC_LD(q + e);
@@ -902,7 +910,10 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = update_of(P, m1[j], f[j]);
       }
-      if (k + kAhead < kK) fetch(mat, col, k + kAhead);
+      if (k + kAhead < kK) {
+        fetch_grad(mat, col, k + kAhead);
+        fetch_mom(mat, col, k + kAhead);
+      }
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const double q = a[8 * i * S + 4 * k];
@@ -915,8 +926,7 @@ __global__ void __launch_bounds__(kThreads, apply_occupancy(NB)) apply_kernel(co
         int nmat;
         int64_t ncol;
         place(x - 1, nmat, ncol);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) fetch(nmat, ncol, k);
+        fetch_first(nmat, ncol, false);
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }

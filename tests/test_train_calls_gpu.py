@@ -9,7 +9,7 @@ import threading
 import pytest
 import torch
 
-from mhc_ops_b200 import _lib, mhc_orthogonalize
+from mhc_ops_b200 import _lib, mhc_muon_step, mhc_orthogonalize
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
@@ -104,3 +104,18 @@ def test_repeated_calls_beside_other_work_return_the_same_bytes(L, R, C):
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("L,R,C", [(64, 24, 4099), (3, 24, 16384), (6, 35, 10005), (2, 63, 4097), (5, 80, 2051),
+                                   (1, 80, 32768), (2, 8, 1000)])
+def test_update_applies_the_momentum_it_wrote(L, R, C):
+    """Without nesterov, decay and parameter the update is -orthogonalised(new momentum), by the same kernels in the
+    same order: the same bits, unless the application read a momentum from before the call.  Odd widths let rows of
+    two CTAs share a cache line."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    m = torch.randn(L, R, C, device="cuda", generator=g)
+    for _ in range(10):
+        grad = torch.randn(L, R, C, device="cuda", generator=g)
+        p = torch.zeros(L, R, C, device="cuda")
+        mhc_muon_step(p, grad, m, 1.0, momentum=0.5, nesterov=False)
+        assert torch.equal(-p, mhc_orthogonalize(m))
