@@ -308,6 +308,12 @@ at::Tensor scratch(size_t nbytes, const at::Device& dev) {
   return at::empty({(int64_t)nbytes}, at::TensorOptions().dtype(at::kByte).device(dev));
 }
 
+// Autograd has to see that these were written.
+void mark_written(at::TensorList tensors) {
+  for (const at::Tensor& t : tensors)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int dtype_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return MHC_BF16;
@@ -508,6 +514,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd_into_cuda(
   }
   b.fwd = in.a;
   check_status(mhc_qk_norm_rope_bwd(&b, at::cuda::getCurrentCUDAStream().stream()), "mhc::qk_norm_rope_bwd");
+  mark_written(grad_out);
   return out;
 }
 
@@ -668,11 +675,8 @@ void muon_step_cuda(at::TensorList params, at::TensorList grads, at::TensorList 
   a.scale = (float)scale;
   a.lr = (float)lr;
   check_status(mhc_muon_step(&a, at::cuda::getCurrentCUDAStream().stream()), "mhc::muon_step_");
-  // autograd has to see that these were written
-  for (const at::Tensor& t : params)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  for (const at::Tensor& t : momenta)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  mark_written(params);
+  mark_written(momenta);
 }
 
 // ----------------------------------------------------------------- Meta kernels (shapes only)

@@ -9,7 +9,7 @@ import threading
 import pytest
 import torch
 
-from mhc_ops_b200 import _lib, mhc_muon_step, mhc_orthogonalize
+from mhc_ops_b200 import _lib, mhc_muon_step, mhc_orthogonalize, mhc_qk_norm_rope_backward
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
@@ -119,3 +119,19 @@ def test_update_applies_the_momentum_it_wrote(L, R, C):
         p = torch.zeros(L, R, C, device="cuda")
         mhc_muon_step(p, grad, m, 1.0, momentum=0.5, nesterov=False)
         assert torch.equal(-p, mhc_orthogonalize(m))
+
+
+def test_autograd_sees_that_gradients_were_written_into_a_saved_tensor():
+    q, f = torch.randn(1, 4, 2, 64, device="cuda"), torch.rand(32, device="cuda")
+    leaf = torch.randn(2, 1, 4, 2, 64, device="cuda", requires_grad=True)
+    buf = torch.zeros(2, 1, 4, 2, 64, device="cuda")
+    y = (leaf * buf).sum()   # saves buf
+    version = buf._version
+    mhc_qk_norm_rope_backward(q, q.clone(), None, f, q.clone(), q.clone(), grad_out=(buf[0], buf[1]))
+    torch.cuda.synchronize()
+    assert buf._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():   # tensors without a version
+        mhc_qk_norm_rope_backward(q, q.clone(), None, f, q.clone(), q.clone(),
+                                  grad_out=(torch.empty_like(q), torch.empty_like(q)))
