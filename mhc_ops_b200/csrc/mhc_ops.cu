@@ -1218,12 +1218,12 @@ int rope_launch_vec(const rope::Params& p, const RopePlan& r, bool backward, cud
   if (backward) {
     auto kernel = rope::bwd_vec_kernel<T, kInter, kGS>;
     constexpr int sums = rope::kWarps * 1024 * (int)sizeof(float), ring = (int)rope::Ring<T, 2>::kBytes;
-    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring + sums));
+    if (int st = set_smem_limit_once(kernel, ring + sums)) return st;
     kernel<<<r.blocks, rope::kThreads, ring + (p.dw_part ? sums : 0), s>>>(p);
   } else {
     auto kernel = rope::fwd_vec_kernel<T, kInter, kGS>;
     constexpr int ring = (int)rope::Ring<T, 1>::kBytes;
-    MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+    if (int st = set_smem_limit_once(kernel, ring)) return st;
     kernel<<<r.blocks, rope::kThreads, ring, s>>>(p);
   }
   return after_launch();
@@ -1334,7 +1334,9 @@ int ortho_check_coeffs(const double* coeffs, int32_t steps, double eps) {
   return MHC_OK;
 }
 
-constexpr int kDefaultSmem = 48 * 1024;   // dynamic shared memory a kernel may have without asking
+// Dynamic shared memory that needs no asking: the default limit less what the
+// kernels below have in static arrays (a few words each), which counts too.
+constexpr int kDefaultSmem = 48 * 1024 - 256;
 
 // A launch that may start while its predecessor in the stream still runs (the
 // kernel waits for what it needs), as clusters of `cluster` CTAs when that is above 1.
@@ -1363,7 +1365,7 @@ template <int NB, int kSP>
 int ortho_iterate_cluster(const OrthoPlan& pl, const ortho::Params& p, cudaStream_t s) {
   auto kernel = ortho::iterate_cluster_kernel<NB, kSP>;
   constexpr int smem = (int)ortho::cluster_smem<NB, kSP>(), cluster = NB / kSP;
-  MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (int st = set_smem_limit_once(kernel, smem)) return st;
   if (cluster > 8) MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return launch_behind(kernel, pl.mats * cluster, 64 * NB, smem, cluster, s, p);
 }
@@ -1406,7 +1408,8 @@ int ortho_iterate(const OrthoPlan& pl, const ortho::Params& p, int sms, [[maybe_
   if constexpr (NB <= ortho::kSmallBlocks) {
     auto kernel = ortho::iterate_small_kernel<NB>;
     constexpr int smem = (int)ortho::small_smem<NB>();
-    if (smem > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if constexpr (smem > kDefaultSmem)
+      if (int st = set_smem_limit_once(kernel, smem)) return st;
     return launch_behind(kernel, pl.mats, 32 * ortho::small_warps(NB), smem, 1, s, p);
   } else {
     // a row block to a CTA while the device holds all the clusters at once, else two
@@ -1425,7 +1428,8 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
       auto fused = vec ? ortho::fused_kernel<NB, T, TO, kMom, true> : ortho::fused_kernel<NB, T, TO, kMom, false>;
       const int smem = (int)ortho::fused_smem<NB>(pl.C);
       // the largest matrix's: a limit that went by C would be lowered under another thread's launch
-      if (int st = set_smem_limit_once(fused, (int)(ortho::fused_fixed_smem<NB>() + ortho::kFusedMatrix))) return st;
+      if (smem > kDefaultSmem)
+        if (int st = set_smem_limit_once(fused, (int)(ortho::fused_fixed_smem<NB>() + ortho::kFusedMatrix))) return st;
       fused<<<pl.mats, ortho::kFusedThreads, smem, s>>>(p, m);
       return after_launch();
     }
@@ -1435,9 +1439,9 @@ int ortho_launch(const OrthoPlan& pl, const ortho::Params& p, const ortho::Mats&
                                    : ortho::apply_smem<NB, TO, false>(pl.apply_warps));
   auto gram = vec ? ortho::gram_kernel<NB, T, kMom, true> : ortho::gram_kernel<NB, T, kMom, false>;
   auto apply = vec ? ortho::apply_kernel<NB, T, TO, kMom, true> : ortho::apply_kernel<NB, T, TO, kMom, false>;
-  if (gs > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(gram, cudaFuncAttributeMaxDynamicSharedMemorySize, gs));
-  if (as > kDefaultSmem) MHC_CUDA_TRY(cudaFuncSetAttribute(apply, cudaFuncAttributeMaxDynamicSharedMemorySize, as));
   int st;
+  if (gs > kDefaultSmem && (st = set_smem_limit_once(gram, gs))) return st;
+  if (as > kDefaultSmem && (st = set_smem_limit_once(apply, as))) return st;   // one size a kernel: 4 warps where they count
   bool clusters = true;
   if constexpr (NB > 8)
     if ((st = ortho_large_clusters(&clusters))) return st;
