@@ -53,9 +53,9 @@ def mhc_orthogonalize(g, coeffs=NEWTON_SCHULZ_COEFFS, eps: float = 1e-7):
     equal matrices, fp32 or bf16, with ``min(rows, cols) <= 80``.
 
     Returns the same kind (a list for a sequence) in the input's type.  Every
-    matrix is treated alone; repeated calls return the same bits.
+    matrix is treated alone; repeated calls return the same bits.  Records no gradient.
     """
-    out = ops.orthogonalize(_list(g, "g"), _coeffs(coeffs), eps)
+    out = ops.untracked(ops.orthogonalize(_list(g, "g"), _coeffs(coeffs), eps))
     return out[0] if torch.is_tensor(g) else out
 
 

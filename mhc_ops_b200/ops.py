@@ -15,7 +15,10 @@ dgamma)``: the reference's ``mhc_backward_manual``
 ``qk_norm_rope`` / ``qk_norm_rope_bwd`` / ``qk_norm_rope_bwd_into``,
 ``orthogonalize`` and ``muon_step_`` are the operators under
 ``mhc_qk_norm_rope``, ``mhc_orthogonalize`` and ``mhc_muon_step``
-(``mhc_ops_b200.qkrope``, ``mhc_ops_b200.muon``), which document them.
+(``mhc_ops_b200.qkrope``, ``mhc_ops_b200.muon``), which document them.  A
+backward pass through one of their results, and a forward-mode tangent on an
+input, raises: the differentiable forms are the autograd Functions of
+``mhc_ops_b200.qkrope``.
 
 The operators run the same kernels as the ctypes API through the C ABI, on the
 current CUDA stream, and have Meta kernels, so FakeTensor tracing
@@ -84,6 +87,12 @@ qk_norm_rope_bwd = _bind("qk_norm_rope_bwd")
 qk_norm_rope_bwd_into = _bind("qk_norm_rope_bwd_into")
 orthogonalize = _bind("orthogonalize")
 muon_step_ = _bind("muon_step_")
+
+
+def untracked(out):
+    """An operator's results without the node that refuses a gradient: the functions that are no autograd Functions
+    return plain tensors whatever their inputs require, as ``mhc_forward_pre`` does."""
+    return [t.detach() for t in out] if out[0].requires_grad else out
 
 
 def check_status() -> None:

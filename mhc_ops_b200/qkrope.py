@@ -46,10 +46,12 @@ def mhc_qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, *,
     ``(2i, 2i + 1)``.  ``q_weight`` / ``k_weight [d]`` are the norms' weights
     (None: ones), ``row_scale [B,S]`` the factor every head of a token is
     multiplied with first.  ``d`` is 1 to 1024.  Returns contiguous ``(q_out,
-    k_out)``, with ``v`` also ``v_out = row_scale * v``.
+    k_out)``, with ``v`` also ``v_out = row_scale * v``.  Records no gradient:
+    ``mhc_qk_norm_rope_fn`` and ``mhc_qkv_norm_rope_fn`` do.
     """
     _check(q)
-    return tuple(ops.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps, interleaved))
+    return tuple(ops.untracked(ops.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps,
+                                                interleaved)))
 
 
 def mhc_qk_norm_rope_backward(q, k, positions, inv_freq, dq_out, dk_out, q_weight=None, k_weight=None, *, v=None,
@@ -70,7 +72,7 @@ def mhc_qk_norm_rope_backward(q, k, positions, inv_freq, dq_out, dk_out, q_weigh
             weight_grads, row_scale_grad)
     count = 2 if v is None else 3
     if grad_out is None:
-        out = ops.qk_norm_rope_bwd(*args)
+        out = ops.untracked(ops.qk_norm_rope_bwd(*args))
         grads, rest = out[:count], out[count:]
     else:
         grads = list(grad_out)
