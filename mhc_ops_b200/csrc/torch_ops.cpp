@@ -30,6 +30,7 @@
 // or mhc::check_status, reports it as an error.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 #include <torch/csrc/autograd/function.h>
@@ -614,18 +615,17 @@ std::vector<at::Tensor> orthogonalize_cuda(at::TensorList g, at::ArrayRef<double
   const Mats m = mats_of(g, "g", true);
   check_sizes(m);
   const int64_t count = (int64_t)m.ptrs.size();
-  at::Tensor stack;
+  // a tensor for each given one: outputs of an operator do not share memory
   std::vector<at::Tensor> out;
-  if (g[0].dim() == 3 || g.size() == 1) {
-    stack = at::empty(g[0].sizes(), g[0].options());
-    out.push_back(stack);
-  } else {
-    stack = at::empty({count, m.rows, m.cols}, g[0].options());
-    out = stack.unbind(0);
+  std::vector<void*> dst;
+  out.reserve(g.size());
+  dst.reserve(m.ptrs.size());
+  for (size_t i = 0; i < g.size(); ++i) {
+    out.push_back(at::detail::empty_cuda(g[i].sizes(), g[i].options()));   // past the dispatcher: lists are long
+    char* p = static_cast<char*>(out.back().data_ptr());
+    const int64_t mats = g[i].dim() == 3 ? count : 1, step = m.rows * m.cols * (int64_t)out.back().element_size();
+    for (int64_t j = 0; j < mats; ++j) dst.push_back(p + j * step);
   }
-  std::vector<void*> dst(m.ptrs.size());
-  const int64_t step = m.rows * m.cols * (int64_t)stack.element_size();
-  for (int64_t i = 0; i < count; ++i) dst[i] = static_cast<char*>(stack.data_ptr()) + i * step;
   const at::Tensor ws = ortho_workspace(m, &a.workspace_bytes, &a.workspace);
   a.in = m.ptrs.data();
   a.out = dst.data();

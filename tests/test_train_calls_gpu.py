@@ -135,3 +135,13 @@ def test_autograd_sees_that_gradients_were_written_into_a_saved_tensor():
     with torch.inference_mode():   # tensors without a version
         mhc_qk_norm_rope_backward(q, q.clone(), None, f, q.clone(), q.clone(),
                                   grad_out=(torch.empty_like(q), torch.empty_like(q)))
+
+
+def test_orthogonalised_matrices_of_a_list_share_no_memory():
+    """An operator's outputs alias nothing: one may be written, or outlive the others, alone."""
+    u = [torch.randn(15, 100, device="cuda") for _ in range(70)]
+    out = mhc_orthogonalize(u)
+    assert len({t.untyped_storage().data_ptr() for t in out}) == len(out)
+    stack = mhc_orthogonalize(torch.stack(u))
+    torch.cuda.synchronize()
+    assert torch.equal(torch.stack(out), stack)
