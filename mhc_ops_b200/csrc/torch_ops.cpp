@@ -358,7 +358,7 @@ at::Tensor unit_inner(const at::Tensor& t) { return t.size(3) <= 1 || t.stride(3
 // The checked inputs of either direction and the tensors that own them.
 struct QkInputs {
   mhc_qk_args a{};
-  at::Tensor q, k, v, inv_freq, q_weight, k_weight, row_scale;
+  at::Tensor q, k, v, inv_freq, q_weight, k_weight, row_scale, positions;
 };
 
 QkInputs qk_inputs(const at::Tensor& q, const at::Tensor& k, const OptTensor& positions, const at::Tensor& inv_freq,
@@ -414,6 +414,7 @@ QkInputs qk_inputs(const at::Tensor& q, const at::Tensor& k, const OptTensor& po
                         "], got ", str(p.sizes()));
       in.a.position_seq_stride = p.stride(0);
     }
+    in.positions = p;
     in.a.positions = p.data_ptr();
     in.a.position_bytes = (int32_t)p.element_size();
   }
@@ -439,6 +440,44 @@ std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
   const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data_ptr());
   return {lo, lo + (uintptr_t)(last + 1) * t.element_size()};
+}
+
+// Whether two [B, S, heads, d] tensors of unit stride along d share a byte.  Equal
+// strides decide it (slices of one packed tensor interleave without meeting): a
+// row of one meets a row of the other when the distance of the bases is off a sum
+// of strides by less than a row.  Other strides leave it open where the spans meet.
+enum class Shared { kNo, kYes, kOpen };
+struct Axis {
+  int64_t stride, a, b;   // bytes; sizes in either tensor
+};
+Shared rows_meet(int64_t gap, const Axis* axis, int n, int64_t row) {
+  if (n == 0) return gap < row && -gap < row ? Shared::kYes : Shared::kNo;
+  int64_t reach = row;   // rows of the inner axes meet only when the rest of the gap is below this
+  for (int i = 1; i < n; ++i) reach += axis[i].stride * (std::max(axis[i].a, axis[i].b) - 1);
+  const int64_t s = axis->stride;
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y != 0 && x < 0); };
+  const int64_t lo = std::max(1 - axis->a, floor_div(-reach - gap, s) + 1), hi = std::min(axis->b - 1, floor_div(reach - gap, s));
+  if (hi - lo > 64) return Shared::kOpen;
+  Shared seen = Shared::kNo;
+  for (int64_t k = lo; k <= hi && seen != Shared::kYes; ++k) {
+    const Shared r = rows_meet(gap + k * s, axis + 1, n - 1, row);
+    if (r != Shared::kNo) seen = r;
+  }
+  return seen;
+}
+Shared shared(const at::Tensor& t, const at::Tensor& u) {
+  const auto a = span_of(t), b = span_of(u);
+  if (a.first >= b.second || b.first >= a.second) return Shared::kNo;
+  Axis axis[3];
+  int n = 0;
+  for (int64_t j = 0; j < 3; ++j) {
+    const int64_t st = t.size(j) > 1 ? t.stride(j) : u.stride(j), su = u.size(j) > 1 ? u.stride(j) : t.stride(j);
+    if (t.size(j) == 1 && u.size(j) == 1) continue;
+    if (st != su || st == 0) return Shared::kOpen;
+    axis[n++] = {st * (int64_t)t.element_size(), t.size(j), u.size(j)};
+  }
+  std::sort(axis, axis + n, [](const Axis& x, const Axis& y) { return x.stride > y.stride; });
+  return rows_meet((int64_t)(b.first - a.first), axis, n, t.size(3) * (int64_t)t.element_size());
 }
 
 }  // namespace
@@ -484,17 +523,26 @@ std::vector<at::Tensor> qk_norm_rope_bwd_into_cuda(
     const at::Tensor& g = grad_out[i];
     check_heads(g, grad_names[i], in.q, inputs[i].size(2));
     TORCH_CHECK_VALUE(g.size(3) == 1 || g.stride(3) == 1, grad_names[i], " must have unit stride along d");
-    for (int64_t j = 0; j < 3; ++j)
+    for (int64_t j = 0; j < 3; ++j) {
       TORCH_CHECK_VALUE(g.stride(j) != 0 || g.size(j) <= 1, grad_names[i], " must not be an expanded tensor");
+      TORCH_CHECK_VALUE(g.stride(j) >= g.size(3) || g.size(j) <= 1, grad_names[i], " overlaps itself");
+    }
     *grad_dst[i] = heads_of(g);
   }
   if (q.numel() > 0)
     for (size_t i = 0; i < count; ++i) {
+      for (size_t j = 0; j < 2 * count; ++j)
+        TORCH_CHECK_VALUE(shared(grad_out[i], j < count ? inputs[j] : ups[j - count]) == Shared::kNo, grad_names[i],
+                          " overlaps an input");
       const auto w = span_of(grad_out[i]);
-      for (size_t j = 0; j < 2 * count; ++j) {
-        const auto r = span_of(j < count ? inputs[j] : ups[j - count]);
-        TORCH_CHECK_VALUE(w.first >= r.second || r.first >= w.second, grad_names[i], " overlaps an input");
-      }
+      for (const at::Tensor& t : {in.q_weight, in.k_weight, in.row_scale, in.inv_freq, in.positions})
+        if (t.defined() && t.numel() > 0) {
+          const auto r = span_of(t);
+          TORCH_CHECK_VALUE(w.first >= r.second || r.first >= w.second, grad_names[i], " overlaps an input");
+        }
+      // of another layout: the caller's word
+      for (size_t j = 0; j < i; ++j)
+        TORCH_CHECK_VALUE(shared(grad_out[i], grad_out[j]) != Shared::kYes, grad_names[i], " overlaps ", grad_names[j]);
     }
   std::vector<at::Tensor> out;
   const auto f = q.options().dtype(at::kFloat);

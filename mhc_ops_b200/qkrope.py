@@ -65,7 +65,9 @@ def mhc_qk_norm_rope_backward(q, k, positions, inv_freq, dq_out, dk_out, q_weigh
     same bits.  ``grad_out`` is an optional ``(dq, dk)`` or ``(dq, dk, dv)`` of
     tensors the gradients are written into, for instance the three slices of
     the packed gradient that the projection's backward takes; they must not
-    overlap the inputs or each other.
+    overlap the inputs, each other or themselves.  Slices of one tensor may lie
+    between one another; a tensor of other strides than an input's has to lie
+    wholly apart from it.
     """
     _check(q)
     args = (q, k, positions, inv_freq, dq_out, dk_out, q_weight, k_weight, v, dv_out, row_scale, eps, interleaved,

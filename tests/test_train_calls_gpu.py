@@ -145,3 +145,83 @@ def test_orthogonalised_matrices_of_a_list_share_no_memory():
     stack = mhc_orthogonalize(torch.stack(u))
     torch.cuda.synchronize()
     assert torch.equal(torch.stack(out), stack)
+
+
+def _grad_call(buf_q, buf_k, q, k, f, dq, dk):
+    out = mhc_qk_norm_rope_backward(q, k, None, f, dq, dk, grad_out=(buf_q, buf_k))
+    torch.cuda.synchronize()
+    return out
+
+
+def test_gradients_that_overlap_are_refused_and_interleaved_ones_are_not():
+    B, S, d = 2, 9, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()   # noqa: E731
+    q, k, dq, dk, f = new(B, S, 4, d), new(B, S, 2, d), new(B, S, 4, d), new(B, S, 2, d), torch.rand(32, device="cuda")
+    want = mhc_qk_norm_rope_backward(q, k, None, f, dq, dk)[:2]
+    pack = new(B, S, 8, d)
+    for a, b in ((pack[:, :, :4], pack[:, :, 3:5]), (pack[:, :, 2:6], pack[:, :, 2:4]),
+                 (pack[:, :, 4:], pack[:, :, 5:7]), (pack[:, :, :4], pack.view(-1)[d // 2:d // 2 + B * S * 8 * d - 8 * d]
+                                                     .as_strided((B, S, 2, d), pack.stride()))):
+        with pytest.raises(ValueError, match="overlaps grad_out dq"):
+            _grad_call(a, b, q, k, f, dq, dk)
+    same = new(B, S, 4, d)
+    with pytest.raises(ValueError, match="overlaps grad_out dq"):
+        mhc_qk_norm_rope_backward(q, q.clone(), None, f, dq, dq.clone(), grad_out=(same, same))
+    with pytest.raises(ValueError, match="overlaps itself"):
+        _grad_call(torch.empty(B * S * 4 * d, dtype=torch.bfloat16, device="cuda").as_strided((B, S, 4, d), (
+            S * 4 * d, 4 * d, d // 2, 1)), new(B, S, 2, d), q, k, f, dq, dk)
+    other = new(B, S, 4, d)
+    with pytest.raises(ValueError, match="overlaps an input"):   # the same memory in another order of axes
+        _grad_call(other.view(B, 4, S, d).transpose(1, 2), new(B, S, 2, d), other, k, f, dq, dk)
+    scale = torch.ones(B * S * 4 * d, device="cuda")
+    with pytest.raises(ValueError, match="overlaps an input"):
+        mhc_qk_norm_rope_backward(q, k, None, f, dq, dk, row_scale=scale[:B * S].view(B, S), grad_out=(
+            scale.view(torch.bfloat16)[:B * S * 4 * d].view(B, S, 4, d), new(B, S, 2, d)))
+    # slices between one another: by heads, by head rows, beside the inputs they belong to, the last token's too
+    _grad_call(pack[:, :, :4], pack[:, :, 4:6], q, k, f, dq, dk)
+    assert torch.equal(pack[:, :, :4], want[0]) and torch.equal(pack[:, :, 4:6], want[1])
+    halves = new(B, S, 4, 2, d)
+    halves[..., 0, :].copy_(q)
+    _grad_call(halves[..., 1, :], new(B, S, 2, d), halves[..., 0, :], k, f, dq, dk)
+    assert torch.equal(halves[..., 1, :], want[0]) and torch.equal(halves[..., 0, :], q)
+    beside = new(B, S, 10, d)
+    beside[:, :, :4].copy_(q)
+    beside[:, :, 4:6].copy_(k)
+    one = beside[:, :, 6:]
+    _grad_call(one, new(B, S, 2, d), beside[:, :, :4], beside[:, :, 4:6], f, dq, dk)
+    assert torch.equal(one, want[0]) and torch.equal(beside[:, :, :4], q) and torch.equal(beside[:, :, 4:6], k)
+    # one sequence of one token: strides of axes of one element say nothing
+    t = new(1, 1, 6, d)
+    r = _grad_call(t[:, :, :4], t[:, :, 4:], q[:1, :1], k[:1, :1], f, dq[:1, :1], dk[:1, :1])
+    assert torch.equal(r[0], want[0][:1, :1]) and torch.equal(r[1], want[1][:1, :1])
+
+
+def test_overlap_of_equal_strides_is_decided_exactly():
+    """Pairs of gradients at random places of one buffer against the sets of their elements; accepted calls write
+    inside the buffer."""
+    import random
+    rng = random.Random(11)
+    buf, f = torch.zeros(20000, device="cuda"), torch.rand(2, device="cuda")
+    met = 0
+    for _ in range(300):
+        B, S, Hq, Hk, d = rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 3), rng.randint(1, 3), 4
+        strides = [d * rng.randint(1, 3)]
+        strides.append(strides[0] * rng.randint(1, 8) + rng.choice([0, 0, d, 3]))
+        strides.append(strides[1] * rng.randint(1, 5) + rng.choice([0, 0, d, 3]))
+        order = rng.choice([(2, 1, 0), (1, 2, 0), (2, 0, 1)])   # which of them batch, sequence and heads take
+        st = tuple(strides[i] for i in order) + (1,)
+        a = buf.as_strided((B, S, Hq, d), st, 4000)
+        b = buf.as_strided((B, S, Hk, d), st, 4000 + rng.randint(-60, 60))
+        places = lambda t: set((torch.arange(20000).as_strided(t.shape, st, t.storage_offset())).flatten().tolist())   # noqa: E731
+        share = bool(places(a) & places(b))
+        met += share
+        q, k = torch.randn(B, S, Hq, d, device="cuda"), torch.randn(B, S, Hk, d, device="cuda")
+        call = lambda: mhc_qk_norm_rope_backward(q, k, None, f, q.clone(), k.clone(), grad_out=(a, b))   # noqa: E731
+        if share:
+            with pytest.raises(ValueError, match="overlaps grad_out dq"):
+                call()
+        else:
+            call()
+    torch.cuda.synchronize()
+    assert 30 < met < 270
