@@ -384,8 +384,8 @@ typedef struct mhc_qk_bwd_args {
 } mhc_qk_bwd_args;
 
 MHC_API int mhc_qk_norm_rope(const mhc_qk_args* args, void* stream);
-/* Workspace bytes of mhc_qk_norm_rope_bwd, 0 without weight gradients.  It
- * depends on the current device's SM count. */
+/* Workspace bytes of mhc_qk_norm_rope_bwd with weight gradients (without them it
+ * takes none).  They depend on the current device's SM count. */
 MHC_API int mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t d, size_t* bytes);
 MHC_API int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* args, void* stream);
 
@@ -418,8 +418,9 @@ typedef struct mhc_ortho_args {
  *   p <- (1 - lr weight_decay) p - lr scale orthogonalised(u).
  * Momenta are fp32, gradients and parameters fp32 or bf16.  lr comes from
  * lr_device (one float in device memory, read when the kernels run) when that
- * is not NULL.  Buffers that overlap return MHC_ERR_OVERLAP (gradients may
- * overlap each other: they are only read). */
+ * is not NULL.  Buffers that overlap return MHC_ERR_OVERLAP, lr_device and what
+ * the call uses of the workspace among them (gradients may overlap each other:
+ * they are only read). */
 typedef struct mhc_muon_args {
   void* const* params;
   const void* const* grads;

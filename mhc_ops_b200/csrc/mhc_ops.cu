@@ -1471,18 +1471,20 @@ struct OrthoLists {
   void* const* outs;
   float* const* moms;   // NULL: orthogonalise only
   int grad_dtype, out_dtype;
+  const float* lr_device;   // NULL, or read by the kernels
 };
 
 // No buffer that is written may share a byte with another one (MHC_ERR_OVERLAP).
-// `same` allows out[i] to be grads[i] itself.
-int ortho_overlap(const OrthoLists& l, int64_t count, size_t elems, bool same) {
+// `same` allows out[i] to be grads[i] itself.  `ws_bytes` is what the call uses of
+// the workspace.
+int ortho_overlap(const OrthoLists& l, int64_t count, size_t elems, bool same, const void* workspace, size_t ws_bytes) {
   struct Span {
     uintptr_t lo, hi;
     bool written;
   };
   std::vector<Span> v;
   try {
-    v.reserve((size_t)count * 3);
+    v.reserve((size_t)count * 3 + 2);
   } catch (...) {   // nothing may be thrown through a C entry point
     return MHC_ERR_LIMIT;
   }
@@ -1495,6 +1497,9 @@ int ortho_overlap(const OrthoLists& l, int64_t count, size_t elems, bool same) {
       v.push_back({m, m + elems * 4, true});
     }
   }
+  const uintptr_t lr = reinterpret_cast<uintptr_t>(l.lr_device), w = reinterpret_cast<uintptr_t>(workspace);
+  if (lr) v.push_back({lr, lr + sizeof(float), false});
+  if (ws_bytes) v.push_back({w, w + ws_bytes, true});
   std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
   uintptr_t end = 0, end_written = 0;   // furthest ends of the spans before
   for (const Span& x : v) {
@@ -1578,13 +1583,13 @@ int ortho_check_lists(const OrthoLists& l, int64_t count, int rows, int cols, bo
         (l.moms && !aligned(l.moms[i], 4)))
       return MHC_ERR_MISALIGNED;
   }
-  if (int st = ortho_overlap(l, count, (size_t)rows * cols, same)) return st;
   const size_t need = ortho_workspace(count, rows, cols, sms);
-  if (need == 0) return MHC_OK;
-  if (!workspace) return MHC_ERR_NULL_POINTER;
-  if (!aligned(workspace, kWsAlign)) return MHC_ERR_MISALIGNED;
-  if (workspace_bytes < need) return MHC_ERR_WORKSPACE_TOO_SMALL;
-  return MHC_OK;
+  if (need > 0) {
+    if (!workspace) return MHC_ERR_NULL_POINTER;
+    if (!aligned(workspace, kWsAlign)) return MHC_ERR_MISALIGNED;
+    if (workspace_bytes < need) return MHC_ERR_WORKSPACE_TOO_SMALL;
+  }
+  return ortho_overlap(l, count, (size_t)rows * cols, same, workspace, need);
 }
 
 // The plan of mhc_query_plan / mhc_query_plan_for (shape already checked).
@@ -2158,7 +2163,7 @@ int mhc_orthogonalize(const mhc_ortho_args* a, void* stream) {
   int sms = 0;
   if ((st = current_sm_count(&sms))) return st;
   if (a->count == 0 || a->rows == 0 || a->cols == 0) return MHC_OK;
-  const OrthoLists l{a->in, a->out, nullptr, a->dtype, a->dtype};
+  const OrthoLists l{a->in, a->out, nullptr, a->dtype, a->dtype, nullptr};
   if ((st = ortho_check_lists(l, a->count, a->rows, a->cols, true, a->workspace, a->workspace_bytes, sms))) return st;
   ortho::Params p{};
   p.steps = a->steps;
@@ -2180,7 +2185,7 @@ int mhc_muon_step(const mhc_muon_args* a, void* stream) {
   if (a->count == 0 || a->rows == 0 || a->cols == 0) return MHC_OK;
   if (!a->momenta) return MHC_ERR_NULL_POINTER;
   if (!aligned(a->lr_device, 4)) return MHC_ERR_MISALIGNED;
-  const OrthoLists l{a->grads, a->params, a->momenta, a->grad_dtype, a->param_dtype};
+  const OrthoLists l{a->grads, a->params, a->momenta, a->grad_dtype, a->param_dtype, a->lr_device};
   if ((st = ortho_check_lists(l, a->count, a->rows, a->cols, false, a->workspace, a->workspace_bytes, sms))) return st;
   ortho::Params p{};
   p.steps = a->steps;

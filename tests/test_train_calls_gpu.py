@@ -225,3 +225,28 @@ def test_overlap_of_equal_strides_is_decided_exactly():
             call()
     torch.cuda.synchronize()
     assert 30 < met < 270
+
+
+def test_learning_rate_and_workspace_may_not_lie_in_what_is_written():
+    p, g, m = (torch.randn(24, 4096, device="cuda") for _ in range(3))
+    lr = torch.full((4,), 0.01, device="cuda")
+    mhc_muon_step(p, g, m, lr[3:])
+    mhc_muon_step(p, g, m, g.view(-1)[5:6])   # only read
+    for inside in (p, m):
+        before = p.clone(), m.clone()
+        with pytest.raises(RuntimeError, match="overlap"):
+            mhc_muon_step(p, g, m, inside.view(-1)[5:6])
+        torch.cuda.synchronize()
+        assert torch.equal(p, before[0]) and torch.equal(m, before[1])
+    lib, vp = _lib.load(), lambda x: ctypes.cast(x, ctypes.c_void_p)
+    n = ctypes.c_size_t(0)
+    assert lib.mhc_ortho_workspace_size(1, 24, 4096, ctypes.byref(n)) == 0 and n.value > 0
+    one = torch.zeros(24 * 4096 * 4 + n.value, dtype=torch.uint8, device="cuda")
+    out = one[:24 * 4096 * 4].view(torch.float32)
+    co = (ctypes.c_double * 3)(1.5, -0.5, 0.0)
+    src, dst = (ctypes.c_void_p * 1)(g.data_ptr()), (ctypes.c_void_p * 1)(out.data_ptr())
+    for ws, want in ((out.data_ptr() + 256, 11), (one.data_ptr() + 24 * 4096 * 4, 0)):
+        a = _lib.OrthoArgs(inp=vp(src), out=vp(dst), count=1, rows=24, cols=4096, dtype=2, steps=1, coeffs=vp(co),
+                           eps=1e-7, workspace=ws, workspace_bytes=n.value)
+        assert lib.mhc_orthogonalize(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == want
+    torch.cuda.synchronize()
