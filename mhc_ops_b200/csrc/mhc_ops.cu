@@ -1156,9 +1156,15 @@ struct RopePlan {
   size_t smem;
 };
 
-// CTAs of the persistent vector kernels at most, and of the other backward: rows
-// of weight-gradient partials.
-int rope_max_blocks(int sms) { return sms * 2; }
+// CTAs of the persistent vector kernels that an SM holds: two, but one of the
+// fp32 backward with weight gradients, whose ring and sums take 96 KB beside 20 KB
+// of static arrays.  With the plan made for two of those, 1184 tokens of 32+8+8
+// heads of 128 took 36.8 us, with one 30.4; 8192 tokens 168 and 164.
+int rope_resident(int dtype, bool weight_grads) { return dtype == MHC_F32 && weight_grads ? 1 : 2; }
+static_assert(2 * (rope::Ring<float, 2>::kBytes + rope::kWarps * 1024 * 4 + 20 * 1024) > 228 * 1024, "two fp32 CTAs fit");
+static_assert(2 * (rope::Ring<uint16_t, 2>::kBytes + rope::kWarps * 1024 * 4 + 21 * 1024) <= 228 * 1024, "two do not fit");
+static_assert(2 * (rope::Ring<float, 2>::kBytes + 21 * 1024) <= 228 * 1024, "two do not fit");
+// CTAs of the other backward at most: rows of weight-gradient partials.
 int rope_max_rows(int sms) { return sms * 4; }
 
 // Dynamic shared memory of the kernels of any width.
@@ -1166,7 +1172,7 @@ constexpr size_t rope_any_smem(int d, int rot, bool backward) {
   return (size_t)rope::kWarps * sizeof(float) * (rot + (backward ? 2 * d : 0));
 }
 
-RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, int sms) {
+RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool backward, bool weight_grads, int sms) {
   RopePlan r{};
   p.x[0] = rope_view(a->q);
   p.x[1] = rope_view(a->k);
@@ -1195,10 +1201,11 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   // Warps per token, the ones that need the fewest steps: rounds of the resident
   // CTAs, each of a warp's share of the groups and about two groups' time for
   // the token's angles and coefficients.  Every warp of a token has a group.
+  const int resident = sms * rope_resident(a->dtype, weight_grads && r.vec);
   int64_t least = 0;
   for (int parts = 1; parts <= rope::kWarps && (parts == 1 || parts <= groups); parts *= 2) {
     const int64_t ctas = (p.T * parts + rope::kWarps - 1) / rope::kWarps;
-    const int64_t rounds = (ctas + rope_max_blocks(sms) - 1) / rope_max_blocks(sms);
+    const int64_t rounds = (ctas + resident - 1) / resident;
     const int64_t steps = rounds * ((groups + parts - 1) / parts + 2);
     if (parts == 1 || steps < least) {
       least = steps;
@@ -1207,7 +1214,7 @@ RopePlan rope_plan(const mhc_qk_args* a, rope::Params& p, bool vec_views, bool b
   }
   const int64_t tok_per_cta = rope::kWarps / p.parts;
   const int64_t want = (p.T + tok_per_cta - 1) / tok_per_cta;
-  r.blocks = (int)std::min<int64_t>(want, r.vec ? rope_max_blocks(sms) : backward ? rope_max_rows(sms) : sms * 16);
+  r.blocks = (int)std::min<int64_t>(want, r.vec ? resident : backward ? rope_max_rows(sms) : sms * 16);
   r.smem = rope_any_smem(p.d, p.rot, backward);
   return r;
 }
@@ -2069,7 +2076,7 @@ int mhc_qk_norm_rope(const mhc_qk_args* a, void* stream) {
                    rope_view_vec(a->q_out, es) && rope_view_vec(a->k_out, es) &&
                    (!a->v.data || rope_view_vec(a->v_out, es));
   rope::Params p{};
-  const RopePlan r = rope_plan(a, p, vec, false, sms);
+  const RopePlan r = rope_plan(a, p, vec, false, false, sms);
   p.out[0] = rope_view(a->q_out);
   p.out[1] = rope_view(a->k_out);
   p.out[2] = rope_view(a->v_out);
@@ -2121,7 +2128,7 @@ int mhc_qk_norm_rope_bwd(const mhc_qk_bwd_args* b, void* stream) {
   if (has_v)
     for (const mhc_heads* h : {&a->v, &b->dv_out, &b->dv}) vec = vec && rope_view_vec(*h, es);
   rope::Params p{};
-  const RopePlan r = rope_plan(a, p, vec, true, sms);
+  const RopePlan r = rope_plan(a, p, vec, true, weights, sms);
   if (weights) {
     if (!b->workspace) return MHC_ERR_NULL_POINTER;
     if (!aligned(b->workspace, 16)) return MHC_ERR_MISALIGNED;
