@@ -3,7 +3,8 @@ has many columns, against float64."""
 import pytest
 import torch
 
-from mhc_ops_b200 import mhc_qk_norm_rope, mhc_qk_norm_rope_backward
+from mhc_ops_b200 import (NEWTON_SCHULZ_COEFFS, mhc_muon_step, mhc_orthogonalize, mhc_qk_norm_rope,
+                          mhc_qk_norm_rope_backward)
 from oracle import train_oracle as O
 from tests.test_qkrope_gpu import HALF, TINY, U32, _inputs, _near, _pairs
 
@@ -54,3 +55,79 @@ def _check_sums(t, rot, eps, interleaved):
                                                          (1, 4999, 3, 1, 50, 50, True)])
 def test_long_rope_calls_against_float64(B, S, Hq, Hk, d, rot, interleaved, dtype):
     _check_sums(_inputs(B, S, Hq, Hk, Hk, d, rot, dtype, seed=S), rot, 1e-3, interleaved)
+
+
+def _decided_bound(u, want, coeffs, eps=1e-7):
+    """What 64-bit sums and one rounding of the result leave, far below a 32-bit Q or application.
+
+    tests/test_muon_gpu.py has the lift of what the Gram sums lose, G^2 of the norm squared per sum |Q||U|.  An
+    accumulator of them takes at most a quarter of the columns (four warps share a chunk at the least), a hundred
+    more additions join the accumulators, and the iteration's products add R terms each, three a step, the first of
+    which are lifted most: (C / 4 + 100 + 4 R) 2^-53 G^2."""
+    from tests.test_muon_gpu import _bound, _gain
+    R, C = sorted(u.shape[-2:])
+    wide = _bound(u, want, coeffs, eps)   # ((R / 2 + 4) u32 + G^2 C 2^-53) sum |Q||U|
+    scale = wide / ((R / 2 + 4) * U32 + _gain(coeffs) ** 2 * C * 2.0 ** -53)
+    return (C / 4 + 100 + 4 * R) * 2.0 ** -53 * _gain(coeffs) ** 2 * scale
+
+
+@pytest.mark.parametrize("L,R,C", [(1, 8, 1024), (2, 24, 512), (1, 24, 4096), (1, 35, 1001), (30, 48, 96), (1, 48, 640),
+                                   (2, 63, 500), (2, 80, 640), (20, 80, 130)])
+def test_orthogonalised_matrix_is_the_rounded_one(L, R, C):
+    from tests.test_muon_gpu import _gradients
+    u = _gradients(L, R, C, seed=R * C)
+    got = mhc_orthogonalize(u)
+    torch.cuda.synchronize()
+    want = O.newton_schulz(u, NEWTON_SCHULZ_COEFFS, 1e-7)
+    _near("O", got, want, _decided_bound(u, want, NEWTON_SCHULZ_COEFFS) + U32 * want.abs())
+
+
+def test_update_of_the_wide_configuration_at_its_full_width():
+    """n = 8, D = 4096: 80 x 32768, two of them (clusters of ten CTAs) and sixteen (of five)."""
+    from tests.test_muon_gpu import _gradients
+    R, C, lr, mu, wd = 80, 32768, 0.02, 0.95, 0.1
+    for L in (2, 16):
+        p, g, m = (_gradients(L, R, C, seed=L + i) for i in range(3))
+        p0, m0 = p.clone(), m.clone()
+        mhc_muon_step(p, g, m, lr, momentum=mu, nesterov=False, weight_decay=wd)
+        torch.cuda.synchronize()
+        for i in sorted({0, 1, L - 1}):
+            m64 = mu * m0[i].double() + (1 - mu) * g[i].double()
+            _near("momentum", m[i], m64, 3 * U32 * (mu * m0[i].double().abs() + (1 - mu) * g[i].double().abs()))
+            want_o = O.newton_schulz(m[i], NEWTON_SCHULZ_COEFFS, 1e-7)
+            lr32, wd32 = (float(torch.tensor(v, dtype=torch.float32)) for v in (lr, wd))
+            keep = 1 - lr32 * wd32
+            want = keep * p0[i].double() - lr32 * want_o
+            # O rounded to 32 bits and multiplied, the decay's factor twice rounded, the sum
+            bound = lr32 * (_decided_bound(m[i], want_o, NEWTON_SCHULZ_COEFFS) + 3 * U32 * want_o.abs())
+            _near("param", p[i], want, bound + 4 * U32 * p0[i].double().abs() + U32 * want.abs())
+
+
+def test_row_factor_carries_a_large_part_of_the_gradient_to_h_in():
+    """h_in's gradient is dqkv w - drow_scale rstd^3 h_in / D, against float64 autograd.
+
+    The upstream gradients are the outputs themselves, so that much of dqkv w lies along h_in and the factor's part
+    takes it away: as large as what is left.  dqkv and drow_scale are right to some 100 u32 of their terms, the sums of
+    512 products in a projection to 512 u32 of theirs at worst, and the terms' sums exceed the sums' norms at most
+    30-fold: 1e-3 of the gradient's norm bounds all of it."""
+    B, S, D, HQ, HK, d, eps = 2, 48, 256, 4, 2, 64, 0.3
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")   # noqa: E731
+    f = (10000.0 ** (-torch.arange(d // 2, device="cuda") / (d // 2))).float()
+    h, w = rnd(B, S, D), rnd((HQ + 2 * HK) * d, D) / D ** 0.5
+    rstd, parts = 1.0 / torch.sqrt((h * h).mean(-1) + 1e-6), (HQ, HK, HK)
+    q, k, v = (h @ w.T).view(B, S, -1, d).split(parts, dim=2)
+    up = mhc_qk_norm_rope(q, k, None, f, v=v, row_scale=rstd, eps=eps)
+    dqkv = torch.empty(B, S, sum(parts), d, device="cuda")
+    out = mhc_qk_norm_rope_backward(q, k, None, f, up[0], up[1], v=v, dv_out=up[2], row_scale=rstd, eps=eps,
+                                    grad_out=dqkv.split(parts, dim=2))
+    direct = dqkv.flatten(2).double() @ w.double()
+    through = -(out[5][..., None] * rstd[..., None] ** 3 * h / D).double()
+    x = h.double().requires_grad_()
+    y = ((x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6)) @ w.double().T).view(B, S, -1, d)
+    angle = O.angles(None, f, B, S)
+    o = [O.norm_rope(t, None, None, angle, eps, False) for t in y.split(parts, dim=2)[:2]] + [y[:, :, HQ + HK:]]
+    want, = torch.autograd.grad(o, x, [t.double() for t in up])
+    assert through.norm() >= 0.5 * want.norm(), float(through.norm() / want.norm())
+    assert (direct + through - want).norm() <= 1e-3 * want.norm()
+    assert (direct - want).norm() >= 0.49 * want.norm()
