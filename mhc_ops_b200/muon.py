@@ -43,9 +43,10 @@ def _list(x, name):
 
 
 def _coeffs(coeffs):
-    if any(len(step) != 3 for step in coeffs):
+    steps = [tuple(step) for step in coeffs]   # once: coeffs may be a generator
+    if any(len(step) != 3 for step in steps):
         raise ValueError("coeffs must be 1 to 16 triples (a, b, c)")
-    return [c for step in coeffs for c in step]
+    return [c for step in steps for c in step]
 
 
 def mhc_orthogonalize(g, coeffs=NEWTON_SCHULZ_COEFFS, eps: float = 1e-7):

@@ -59,3 +59,10 @@ def test_autograd_function_traces_under_fake_tensors():
     names = [str(n.target) for n in graph.graph.nodes if n.op == "call_function"]
     assert sum("mhc.qk_norm_rope.default" in n for n in names) == 1
     assert sum("mhc.qk_norm_rope_bwd" in n for n in names) == 1
+
+
+def test_coefficients_may_come_from_a_generator():
+    from mhc_ops_b200.muon import _coeffs
+    assert _coeffs((a, -0.5, 0.0) for a in (1.5, 2.0)) == [1.5, -0.5, 0.0, 2.0, -0.5, 0.0]
+    with pytest.raises(ValueError, match="triples"):
+        _coeffs(iter([(1.0, 2.0)]))
