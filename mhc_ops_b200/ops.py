@@ -47,7 +47,8 @@ def lib_path() -> str:
 
 
 def load() -> None:
-    """Register the ``mhc`` operators (once); raises if the library is not built."""
+    """Register the ``mhc`` operators (once); raises if the library is not built.  Call it before a program whose
+    first use of them is inside ``torch.compile``, which cannot trace the loading."""
     global _loaded
     if _loaded:
         return
@@ -57,6 +58,8 @@ def load() -> None:
                 raise RuntimeError(f"libmhc_torch.so not found at {_LIB_PATH}; build it with "
                                    "`python -m mhc_ops_b200.build` (there is no fallback)")
             torch.ops.load_library(_LIB_PATH)
+            for name in _BOUND:
+                globals()[name] = getattr(torch.ops.mhc, name).default
             _loaded = True
 
 
@@ -72,21 +75,33 @@ def bwd(x, phi, alpha, inv_rms, h_mix, h_pre, h_post, dh_in, dh_post, dh_res, ga
                              norm_eps, hc_eps)
 
 
-def _bind(name):
-    """The operator's call without the overload lookup; looked up at the first call."""
-    def first(*args):
-        load()
-        op = getattr(torch.ops.mhc, name).default
-        globals()[name] = op
-        return op(*args)
-    return first
+# The operators' calls without the overload lookup; load() puts them in place of these, which serve a first call.
+_BOUND = ("qk_norm_rope", "qk_norm_rope_bwd", "qk_norm_rope_bwd_into", "orthogonalize", "muon_step_")
 
 
-qk_norm_rope = _bind("qk_norm_rope")
-qk_norm_rope_bwd = _bind("qk_norm_rope_bwd")
-qk_norm_rope_bwd_into = _bind("qk_norm_rope_bwd_into")
-orthogonalize = _bind("orthogonalize")
-muon_step_ = _bind("muon_step_")
+def qk_norm_rope(*args):
+    load()
+    return torch.ops.mhc.qk_norm_rope.default(*args)
+
+
+def qk_norm_rope_bwd(*args):
+    load()
+    return torch.ops.mhc.qk_norm_rope_bwd.default(*args)
+
+
+def qk_norm_rope_bwd_into(*args):
+    load()
+    return torch.ops.mhc.qk_norm_rope_bwd_into.default(*args)
+
+
+def orthogonalize(*args):
+    load()
+    return torch.ops.mhc.orthogonalize.default(*args)
+
+
+def muon_step_(*args):
+    load()
+    return torch.ops.mhc.muon_step_.default(*args)
 
 
 def untracked(out):
