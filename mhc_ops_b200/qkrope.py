@@ -41,8 +41,8 @@ def mhc_qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, *,
     ``q [B,S,Hq,d]``, ``k [B,S,Hk,d]`` and the optional ``v [B,S,Hv,d]`` may be
     views of one packed projection.  ``positions`` are int32/int64 ``[B,S]`` or
     ``[S]`` (None: 0 .. S-1), of any value below 2^31 in magnitude;
-    ``inv_freq [rot/2]`` the angles per position of the ``rot <= d`` leading
-    elements that turn, in pairs ``(i, i + rot/2)`` or, ``interleaved``,
+    ``inv_freq [rot/2]``, taken in fp32, the angles per position of the
+    ``rot <= d`` leading elements that turn, in pairs ``(i, i + rot/2)`` or, ``interleaved``,
     ``(2i, 2i + 1)``.  ``q_weight`` / ``k_weight [d]`` are the norms' weights
     (None: ones), ``row_scale [B,S]`` the factor every head of a token is
     multiplied with first.  ``d`` is 1 to 1024.  Returns contiguous ``(q_out,
@@ -76,6 +76,14 @@ def mhc_qk_norm_rope_backward(q, k, positions, inv_freq, dq_out, dk_out, q_weigh
     if grad_out is None:
         out = ops.untracked(ops.qk_norm_rope_bwd(*args))
         grads, rest = out[:count], out[count:]
+    elif torch.compiler.is_compiling():
+        # a traced operator that writes into given tensors may not return others: one copy more
+        out = ops.untracked(ops.qk_norm_rope_bwd(*args))
+        grads, rest = list(grad_out), out[count:]
+        if len(grads) != count:
+            raise ValueError(f"grad_out must hold {count} tensors")
+        for t, g in zip(grads, out):
+            t.copy_(g)
     else:
         grads = list(grad_out)
         rest = ops.qk_norm_rope_bwd_into(*args, grads)

@@ -9,10 +9,12 @@ import warnings
 import pytest
 import torch
 
-from mhc_ops_b200 import mhc_muon_step, mhc_orthogonalize, ops
+from mhc_ops_b200 import (mhc_muon_step, mhc_orthogonalize, mhc_qk_norm_rope, mhc_qk_norm_rope_backward,
+                          mhc_qkv_norm_rope_fn, ops)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
+B, S, HQ, HK, d = 2, 30, 4, 2, 64
 
 
 def _compiled(fn):
@@ -29,6 +31,40 @@ def _same(got, want):
 def _leaf(*shape, dtype=torch.float32, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     return torch.randn(*shape, generator=g, device="cuda").to(dtype).requires_grad_()
+
+
+F = lambda: torch.rand(d // 2, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))   # noqa: E731
+
+
+def test_packed_projection_and_its_gradients():
+    def fn(qkv, f, wq, wk, sc):
+        q, k, v = mhc_qkv_norm_rope_fn(qkv, HQ, HK, None, f, wq, wk, row_scale=sc)
+        return (q.float() ** 2).sum() + k.float().sum() * 3 + (v.float() ** 3).sum()
+
+    qkv, sc, wq = _leaf(B, S, HQ + 2 * HK, d, dtype=torch.bfloat16), _leaf(B, S, seed=1), _leaf(d, seed=2)
+    wk = _leaf(d, seed=3)
+    leaves = (qkv, sc, wq, wk)
+    want = torch.autograd.grad(fn(qkv, F(), wq, wk, sc), leaves)
+    _same(torch.autograd.grad(_compiled(fn)(qkv, F(), wq, wk, sc), leaves), want)
+
+
+def test_calls_by_hand():
+    def by_hand(q, k, f, up_q, up_k, w):
+        y, z = mhc_qk_norm_rope(q, k, None, f, w)
+        pack = torch.empty(B, S, HQ + HK, d, device="cuda", dtype=q.dtype)
+        out = mhc_qk_norm_rope_backward(q, k, None, f, up_q, up_k, w, grad_out=pack.split((HQ, HK), dim=2))
+        apart = mhc_qk_norm_rope_backward(q, k, None, f, up_q, up_k, w)
+        return y, z, pack * 1, out[0] * 1, out[3], apart[0], apart[3]
+
+    rnd = lambda h, s: _leaf(B, S, h, d, dtype=torch.bfloat16, seed=s).detach()   # noqa: E731
+    args = (rnd(HQ, 1), rnd(HK, 2), F(), rnd(HQ, 3), rnd(HK, 4), _leaf(d, seed=5).detach())
+    _same(_compiled(by_hand)(*args), by_hand(*args))
+
+    def short(q, k, f):
+        return mhc_qk_norm_rope_backward(q, k, None, f, q, k, grad_out=(torch.empty_like(q),))
+
+    with pytest.raises(Exception, match="hold 2"):
+        _compiled(short)(args[0], args[1], args[2])
 
 
 def test_update_and_orthogonalisation_of_lists():
