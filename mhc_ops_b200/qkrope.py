@@ -150,14 +150,22 @@ class MHCQKVNormRopeFunction(torch.autograd.Function):
                 None)
 
 
+def _other(t, u):
+    """``t``, as a view where it is ``u`` itself: ``torch.compile`` keeps one of the gradients of a tensor that an
+    autograd Function takes twice."""
+    return t.view_as(t) if t is not None and t is u else t
+
+
 def mhc_qk_norm_rope_fn(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, v=None, row_scale=None,
                         eps: float = 1e-6, interleaved: bool = False):
     """Differentiable ``mhc_qk_norm_rope``."""
+    k, v, k_weight = _other(k, q), _other(_other(v, q), k), _other(k_weight, q_weight)
     return MHCQKNormRopeFunction.apply(q, k, positions, inv_freq, q_weight, k_weight, v, row_scale, eps, interleaved)
 
 
 def mhc_qkv_norm_rope_fn(qkv, q_heads: int, k_heads: int, positions, inv_freq, q_weight=None, k_weight=None, *,
                          row_scale=None, eps: float = 1e-6, interleaved: bool = False):
     """Differentiable ``mhc_qk_norm_rope`` on a packed projection ``[B,S,Hq+2Hk,d]``: returns ``(q, k, v)``."""
+    k_weight = _other(k_weight, q_weight)
     return MHCQKVNormRopeFunction.apply(qkv, q_heads, k_heads, positions, inv_freq, q_weight, k_weight, row_scale,
                                         eps, interleaved)

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from mhc_ops_b200 import (mhc_muon_step, mhc_orthogonalize, mhc_qk_norm_rope, mhc_qk_norm_rope_backward,
-                          mhc_qkv_norm_rope_fn, ops)
+                          mhc_qk_norm_rope_fn, mhc_qkv_norm_rope_fn, ops)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
@@ -36,16 +36,32 @@ def _leaf(*shape, dtype=torch.float32, seed=0):
 F = lambda: torch.rand(d // 2, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))   # noqa: E731
 
 
-def test_packed_projection_and_its_gradients():
+@pytest.mark.parametrize("twice", [False, True])
+def test_packed_projection_and_its_gradients(twice):
+    """With one weight for queries and keys its gradient is the sum of both."""
     def fn(qkv, f, wq, wk, sc):
         q, k, v = mhc_qkv_norm_rope_fn(qkv, HQ, HK, None, f, wq, wk, row_scale=sc)
         return (q.float() ** 2).sum() + k.float().sum() * 3 + (v.float() ** 3).sum()
 
     qkv, sc, wq = _leaf(B, S, HQ + 2 * HK, d, dtype=torch.bfloat16), _leaf(B, S, seed=1), _leaf(d, seed=2)
-    wk = _leaf(d, seed=3)
-    leaves = (qkv, sc, wq, wk)
+    wk = wq if twice else _leaf(d, seed=3)
+    leaves = (qkv, sc, wq) if twice else (qkv, sc, wq, wk)
     want = torch.autograd.grad(fn(qkv, F(), wq, wk, sc), leaves)
     _same(torch.autograd.grad(_compiled(fn)(qkv, F(), wq, wk, sc), leaves), want)
+
+
+def test_one_tensor_for_queries_keys_and_values():
+    def fn(q, k, v, f, w, u):
+        q, k, v = mhc_qk_norm_rope_fn(q, k, None, f, w, u, v=v)
+        return (q.float() ** 3).sum() + k.float().sum() * 3 + (v.float() ** 2).sum()
+
+    x, w = _leaf(B, S, HQ, d), _leaf(d, seed=2)
+    want = torch.autograd.grad(fn(x, x, x, F(), w, w), (x, w))
+    apart = [t.detach().clone().requires_grad_() for t in (x, x, x, w, w)]
+    parts = torch.autograd.grad(fn(*apart[:3], F(), *apart[3:]), apart)
+    for got, p in ((want[0], parts[:3]), (want[1], parts[3:])):   # the same terms, added in 32 bits
+        assert (got - sum(t.double() for t in p)).abs().max() <= 2 ** -22 * sum(t.abs().max() for t in p)
+    _same(torch.autograd.grad(_compiled(fn)(x, x, x, F(), w, w), (x, w)), want)
 
 
 def test_calls_by_hand():
