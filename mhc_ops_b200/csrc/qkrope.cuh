@@ -650,10 +650,10 @@ __global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const __grid_const
         unit = col / 16;
         e = col % 16;
       }
-      float sum = 0.f;
+      double sum = 0.0;   // 64 lanes' sums one behind the other: in 32 bits half of the gradient's error
       for (int w = 0; w < kWarps; ++w)
-        for (int k = 0; k < (32 >> kGS); ++k) sum += dyn[w * 1024 + side * 512 + e * 32 + (k << kGS) + unit];
-      MHC_ST(P.dw_part + (int64_t)blockIdx.x * 2 * P.d + i, sum);
+        for (int k = 0; k < (32 >> kGS); ++k) sum += (double)dyn[w * 1024 + side * 512 + e * 32 + (k << kGS) + unit];
+      MHC_ST(P.dw_part + (int64_t)blockIdx.x * 2 * P.d + i, (float)sum);
     }
   }
 }
@@ -852,18 +852,19 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const __grid_constant
 // columns a CTA, every warp an eighth of the rows.
 __global__ void __launch_bounds__(kThreads) bwd_weights_kernel(const float* __restrict__ part, int rows, int d,
                                                                float* __restrict__ dwq, float* __restrict__ dwk) {
-  __shared__ float acc[kWarps][kFinCols];
+  __shared__ double acc[kWarps][kFinCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * kFinCols + lane;
-  float sum = 0.f;
+  double sum = 0.0;
   if (col < 2 * d)
-    for (int r = warp; r < rows; r += kWarps) sum += MHC_LDG(part + (int64_t)r * 2 * d + col);
+    for (int r = warp; r < rows; r += kWarps) sum += (double)MHC_LDG(part + (int64_t)r * 2 * d + col);
   acc[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && col < 2 * d) {
-    float v = 0.f;
+    double sums = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += acc[w][lane];
+    for (int w = 0; w < kWarps; ++w) sums += acc[w][lane];
+    const float v = (float)sums;
     if (col < d) {
       if (dwq) MHC_ST(dwq + col, v);
     } else if (dwk) {

@@ -57,6 +57,24 @@ def test_long_rope_calls_against_float64(B, S, Hq, Hk, d, rot, interleaved, dtyp
     _check_sums(_inputs(B, S, Hq, Hk, Hk, d, rot, dtype, seed=S), rot, 1e-3, interleaved)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_weight_gradients_of_many_rows_keep_their_last_bit(seed):
+    """Some 4,700 rows a sum: lanes add a few of them in 32 bits, everything behind the lanes is added in 64.
+
+    What is left are the rounding of a lane's terms and sums, of a CTA's row and of the result, at most u32 of each
+    layer's terms and of independent signs: sqrt(3) u32 of the gradient's norm, and with the terms' own errors, which
+    average out over the rows, below 2 u32."""
+    B, S, d, eps = 2, 333, 64, 1e-6
+    t = _inputs(B, S, 7, 1, 1, d, d, torch.float32, seed=100 + seed)
+    g = mhc_qk_norm_rope_backward(t["q"], t["k"], t["positions"], t["inv_freq"], t["dq"], t["dk"], t["wq"], t["wk"],
+                                  eps=eps)
+    torch.cuda.synchronize()
+    angle = O.angles(t["positions"], t["inv_freq"], B, S)
+    for x, dy, w, got in ((t["q"], t["dq"], t["wq"], g[3]), (t["k"], t["dk"], t["wk"], g[4])):
+        want = O.norm_rope_backward(x.double(), dy.double(), w.double(), None, angle, eps, False)[1]
+        assert (got - want).norm() <= 2 * U32 * want.norm(), float((got - want).norm() / want.norm() / U32)
+
+
 def _decided_bound(u, want, coeffs, eps=1e-7):
     """What 64-bit sums and one rounding of the result leave, far below a 32-bit Q or application.
 
