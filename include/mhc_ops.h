@@ -456,7 +456,10 @@ MHC_API uint64_t mhc_launch_count(void);
 /* Version of this ABI (major*10000 + minor*100 + patch).  1.1.0 added the
  * post-op and the device-free plan queries, 1.2.0 the backward that
  * recomputes the forward's intermediates and mhc_fwd_ex, 1.3.0 the
- * debug-bounds entry points, 1.4.0 mhc_query_bwd_grid. */
+ * debug-bounds entry points, 1.4.0 mhc_query_bwd_grid.  The operators for
+ * queries and keys and for updates of phi came in without another number: a
+ * library has them when mhc_status_string(MHC_ERR_OVERLAP) is not "unknown mhc
+ * status". */
 MHC_API int mhc_abi_version(void);
 
 /* Debug-bounds builds (compiled with -DMHC_DEBUG_BOUNDS: lib/libmhc_ops_dbg.so

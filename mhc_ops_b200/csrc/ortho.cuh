@@ -786,11 +786,11 @@ __global__ void __launch_bounds__(64 * NB) iterate_cluster_kernel(const __grid_c
 // products run.  The next columns' first rows are loaded before this step's
 // results are stored.  With few rows all of a step's loads are in registers at
 // once instead, and other warps' work covers them.
-// 64 x 24 x 16384, update: 76 us, 403 MB at 5.3 TB/s.  8 x 80 x 32768: 150 us,
-// 1.68 G multiply-adds, 61% of the matrix pipe's rate; taking out the stores, the
+// 64 x 24 x 16384, update: 77 us, 403 MB at 5.2 TB/s.  8 x 80 x 32768: 141 us,
+// 1.68 G multiply-adds, 65% of the matrix pipe's rate; taking out the stores, the
 // parameters or the loads gains 10 us each, so no single one of them holds it.
-// Turns at the pipe for the two warps that share one (288 us a call instead of
-// 274) and 16 warps of half the rows each (283) were slower.
+// Turns at the pipe for the two warps that share one (288 us a call where this
+// took 274) and 16 warps of half the rows each (283) were slower.
 constexpr int apply_occupancy(int NB) { return NB <= 3 ? 2 : 1; }
 // row loads in flight; element by element they are all that hides their latency
 constexpr int apply_ahead(int NB, bool vec) { return NB <= 3 || (!vec && NB == 5) ? 2 * NB : !vec && NB == 6 ? 6 : 4; }

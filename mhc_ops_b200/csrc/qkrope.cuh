@@ -462,10 +462,15 @@ __global__ void __launch_bounds__(kThreads, 2) fwd_vec_kernel(const __grid_const
 
 // Backward.  Each lane keeps the weight gradients of its 16 elements: in
 // registers over a side's head groups, in its own shared-memory slots over
-// tokens.  The CTA's warps are added in warp order and the CTA's row written for
-// the finalize kernel, so repeated calls give the same bits.  113 us for the
-// forward's tokens, 604 MB at 5.3 TB/s; its sums, angles and weights fill 128
-// registers, and of 16 warps an SM 57% of the issue slots are used.
+// tokens.  The CTA's warps are added in warp order, in 64 bits, and the CTA's row
+// written for the finalize kernel, so repeated calls give the same bits.  113 us
+// for the forward's tokens, 604 MB at 5.3 TB/s (119 to 124 a call with the
+// finalize kernel); its sums, angles and weights fill 128 registers, and of 16
+// warps an SM 57% of the issue slots are used.  Wide heads, few to a token, wait
+// instead: 67 us for 8191 tokens of 16+2 heads of 256, 226 MB at 3.4 TB/s, 44% of
+// the slots, three tenths of the stalls on shared memory and conversions (the angles
+// and sums of every token, which 18 heads share) and a quarter on the
+// instruction before.
 template <class T, bool kInter, int kGS>
 __global__ void __launch_bounds__(kThreads, 2) bwd_vec_kernel(const __grid_constant__ Params P) {
   __shared__ __align__(16) float sw[2][512];
@@ -848,8 +853,8 @@ __global__ void __launch_bounds__(kThreads) bwd_any_kernel(const __grid_constant
     }
 }
 
-// Weight gradients: the CTAs' rows [parts][2 d] added in a fixed order, 32
-// columns a CTA, every warp an eighth of the rows.
+// Weight gradients: the CTAs' rows [parts][2 d] added in 64 bits in a fixed
+// order, 32 columns a CTA, every warp an eighth of the rows.
 __global__ void __launch_bounds__(kThreads) bwd_weights_kernel(const float* __restrict__ part, int rows, int d,
                                                                float* __restrict__ dwq, float* __restrict__ dwk) {
   __shared__ double acc[kWarps][kFinCols];
