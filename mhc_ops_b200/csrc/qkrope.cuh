@@ -85,14 +85,6 @@ template <class T>
 struct Raw8 {
   static constexpr int kWords = sizeof(T) * 8 / 16;
   uint4 w[kWords];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = MHC_LDG(reinterpret_cast<const uint4*>(p) + i);
-  }
   __device__ __forceinline__ void unpack(float2 (&f)[4]) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
@@ -350,7 +342,7 @@ __device__ __forceinline__ bool lane_unit(const Params& P, int lane, int& u, int
 // token and side, so that a pair costs three packed instructions each way.
 // Memory bounds it: 72 us at B=4, S=4096, 32+8+8 heads of 128, bf16, 403 MB at
 // 5.6 TB/s (a copy of the same rows: 65 us).  A few tokens are bound by the
-// launch: 4.7 us for one.
+// launch: 5.0 us for one.
 template <class T, bool kInter, int kGS>
 __global__ void __launch_bounds__(kThreads, 2) fwd_vec_kernel(const __grid_constant__ Params P) {
   __shared__ __align__(16) float sw[2][512];
